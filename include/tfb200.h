@@ -88,6 +88,10 @@ extern "C" {
  * (0, 8, 16 or 24; with TF_ATTN_EXP_F16X2: 0 or 16; fp16 operands only) */
 #define TF_ATTN_FMA_EXP_SHIFT 8
 
+/* tf_rotary / tf_rotary_append flags */
+#define TF_ROTARY_INTERLEAVED 1 /* pairs (2i, 2i + 1); default (i, i + rot/2) */
+#define TF_ROTARY_BF16 2        /* bf16 operands (default fp16) */
+
 /* ABI version, bumped on any signature change. */
 int tf_abi_version(void);
 
@@ -281,6 +285,38 @@ int tf_flash_fwd(const void* q, const void* k, const void* v, int64_t ld_q, int6
 int tf_attn_merge(float* o_acc, float* lse_acc, const float* o_part, const float* lse_part, int64_t ld,
                   int64_t bs, void* out16, int64_t ld16, int64_t bs16, int64_t batch, int64_t heads,
                   int64_t seq_q, int64_t head_dim, void* stream);
+
+/* Rotary positions: in every head the pair (a, b) = (i, i + rot/2), or
+ * (2i, 2i + 1) with TF_ROTARY_INTERLEAVED, i < rot/2, becomes
+ *   m * (x_a cos t - x_b sin t, x_a sin t + x_b cos t),  t = positions[token] * freqs[i]
+ * and elements rot .. head_dim - 1 are copied; the angle is formed in 64 bits,
+ * the rotation in fp32, one rounding to the 16-bit type. q: token and head
+ * strides q_ts, q_hs, unit inner stride; likewise q_out, k, k_out (heads and
+ * kv_heads of them; either count may be 0). Outputs may be their inputs (in
+ * place) but must not overlap them otherwise. positions int64 [tokens], any
+ * sign (negated positions give the transpose); freqs fp64 [rot / 2].
+ * head_dim 2 .. 256, rot even. Any strides and 2-byte alignment; multiples of
+ * 8 elements and 16-byte bases are fastest.
+ * No reference counterpart: the reference's encoder has no positions; this
+ * stands between its QKV projection and its attention
+ * (torch_transformer_benchmark.py:4138-4161). */
+int tf_rotary(const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs, const void* k,
+              int64_t k_ts, int64_t k_hs, void* k_out, int64_t ko_ts, int64_t ko_hs, const int64_t* positions,
+              const double* freqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rot,
+              float mscale, int flags, void* stream);
+
+/* tf_rotary whose rotated keys, and the values v, go into a paged cache:
+ * token t's key head h to k_cache + page * c_ps + row * c_ts + h * c_hs with
+ * page = slots[t] / page_size, row = slots[t] % page_size, its value to the
+ * same place of v_cache. slots int64 [tokens], distinct where not negative; a
+ * negative slot writes nothing, one past num_pages * page_size writes nothing
+ * and sets device code 108 (tf_device_status). No reference counterpart. */
+int tf_rotary_append(const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs,
+                     const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
+                     const int64_t* positions, const double* freqs, void* k_cache, void* v_cache, int64_t c_ps,
+                     int64_t c_ts, int64_t c_hs, int64_t num_pages, int64_t page_size, const int64_t* slots,
+                     int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rot, float mscale,
+                     int flags, void* stream);
 
 #ifdef __cplusplus
 }

@@ -51,6 +51,9 @@ TF_ATTN_EXP_F16X2 = 4
 TF_ATTN_BF16 = 8
 TF_ATTN_ROUND_SCORES = 16
 
+TF_ROTARY_INTERLEAVED = 1
+TF_ROTARY_BF16 = 2
+
 # every symbol include/tfb200.h declares, with its ctypes signature
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -69,6 +72,10 @@ SIGNATURES = {
     "tf_ln_ready": ([_P, _P, _P, _F, _P, _I64, _I64, _I, _P, _P, _P], _I),
     "tf_flash_fwd": ([_P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P,
                       _I64, _I64, _I64, _I64, _I64, _F, _I64, _I64, _I, _P], _I),
+    "tf_rotary": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P,
+                   _I64, _I64, _I64, _I64, _I64, _F, _I, _P], _I),
+    "tf_rotary_append": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P,
+                          _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _F, _I, _P], _I),
     "tf_attn_merge": ([_P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P], _I),
     "tf_gemm_splitk_workspace": ([_I64, _I64, _I64, _I], _I64),
     "tf_gemm_splitk": ([_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _P, _I64, _P], _I),

@@ -504,4 +504,97 @@ int tf_attn_merge(float* o_acc, float* lse_acc, const float* o_part, const float
   return tfb::attn_merge(a, as_stream(stream));
 }
 
+// The serving entry points check their arguments before they look for a
+// device, so a malformed call gets the same status on any host.
+static inline void clear_message() {
+  tfb::g_msg[0] = '\0';
+  tfb::g_code = TF_OK;
+}
+
+static int narrow_dims(const char* fn, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rot) {
+  for (int64_t v : {heads, kv_heads, head_dim, rot})
+    if (v < 0 || v > (1 << 20)) return set_error(TF_ERR_SHAPE, "%s: sizes out of range", fn);
+  return TF_OK;
+}
+
+static int rotary_common(const char* fn, tfb::RotaryArgs& a, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                         int64_t rot, int flags, void* stream) {
+  clear_message();
+  if (flags & ~(TF_ROTARY_INTERLEAVED | TF_ROTARY_BF16)) return set_error(TF_ERR_SHAPE, "%s: unknown flags", fn);
+  int rc = narrow_dims(fn, heads, kv_heads, head_dim, rot);
+  if (rc) return rc;
+  a.heads = static_cast<int>(heads);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.head_dim = static_cast<int>(head_dim);
+  a.rot = static_cast<int>(rot);
+  a.interleaved = (flags & TF_ROTARY_INTERLEAVED) != 0;
+  a.bf16 = (flags & TF_ROTARY_BF16) != 0;
+  rc = tfb::rotary_check(a, fn);
+  if (rc) return rc;
+  rc = begin_call();
+  if (rc) return rc;
+  return tfb::rotary(a, as_stream(stream));
+}
+
+int tf_rotary(const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs, const void* k,
+              int64_t k_ts, int64_t k_hs, void* k_out, int64_t ko_ts, int64_t ko_hs, const int64_t* positions,
+              const double* freqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rot,
+              float mscale, int flags, void* stream) {
+  tfb::RotaryArgs a = {};
+  a.q = q;
+  a.q_ts = q_ts;
+  a.q_hs = q_hs;
+  a.q_out = q_out;
+  a.qo_ts = qo_ts;
+  a.qo_hs = qo_hs;
+  a.k = k;
+  a.k_ts = k_ts;
+  a.k_hs = k_hs;
+  a.k_out = k_out;
+  a.ko_ts = ko_ts;
+  a.ko_hs = ko_hs;
+  a.positions = positions;
+  a.freqs = freqs;
+  a.tokens = tokens;
+  a.mscale = mscale;
+  return rotary_common("tf_rotary", a, heads, kv_heads, head_dim, rot, flags, stream);
+}
+
+int tf_rotary_append(const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int64_t qo_ts, int64_t qo_hs,
+                     const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
+                     const int64_t* positions, const double* freqs, void* k_cache, void* v_cache, int64_t c_ps,
+                     int64_t c_ts, int64_t c_hs, int64_t num_pages, int64_t page_size, const int64_t* slots,
+                     int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rot, float mscale,
+                     int flags, void* stream) {
+  clear_message();
+  if (tokens > 0 && (k_cache == nullptr || v_cache == nullptr))
+    return set_error(TF_ERR_SHAPE, "tf_rotary_append: null cache");
+  tfb::RotaryArgs a = {};
+  a.q = q;
+  a.q_ts = q_ts;
+  a.q_hs = q_hs;
+  a.q_out = q_out;
+  a.qo_ts = qo_ts;
+  a.qo_hs = qo_hs;
+  a.k = k;
+  a.k_ts = k_ts;
+  a.k_hs = k_hs;
+  a.v = v;
+  a.v_ts = v_ts;
+  a.v_hs = v_hs;
+  a.positions = positions;
+  a.freqs = freqs;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.c_ps = c_ps;
+  a.c_ts = c_ts;
+  a.c_hs = c_hs;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.slots = slots;
+  a.tokens = tokens;
+  a.mscale = mscale;
+  return rotary_common("tf_rotary_append", a, heads, kv_heads, head_dim, rot, flags, stream);
+}
+
 }  // extern "C"

@@ -33,6 +33,7 @@ enum DeviceError : int {
   kDevTimeoutDrain = 105,
   kDevTimeoutProbe = 106,  // tf_test_wait_timeout: the wait made to run out
   kDevReadyCount = 107,    // a row group's ready count never reached (or overshot) its target
+  kDevBadIndex = 108,      // a slot, page, length or offset outside the arrays it indexes (nothing was accessed there)
 };
 
 // Wall-time bound of a single wait: far above any legitimate wait (the

@@ -146,6 +146,62 @@ struct MergeArgs {
 
 int attn_merge(const MergeArgs& a, cudaStream_t stream);
 
+// rotary positions (rotary.cu); k_cache non-null: keys and values to the cache
+struct RotaryArgs {
+  const void* q;
+  long long q_ts, q_hs;  // token and head strides, elements
+  void* q_out;
+  long long qo_ts, qo_hs;
+  const void* k;
+  long long k_ts, k_hs;
+  void* k_out;
+  long long ko_ts, ko_hs;
+  const void* v;
+  long long v_ts, v_hs;
+  const int64_t* positions;
+  const double* freqs;
+  void* k_cache;
+  void* v_cache;
+  long long c_ps, c_ts, c_hs;  // page, token and head strides of both caches
+  long long num_pages, page_size;
+  const int64_t* slots;
+  long long tokens;
+  int heads, kv_heads, head_dim, rot;
+  float mscale;
+  int interleaved, bf16;
+};
+
+// Argument checks that need no device (the C entry makes them first).
+int rotary_check(const RotaryArgs& a, const char* fn);
+int rotary(const RotaryArgs& a, cudaStream_t stream);
+
+// attention of new tokens over a paged cache
+struct PagedArgs {
+  const void* q;
+  long long q_ts, q_hs;
+  const void* k_cache;
+  const void* v_cache;
+  long long c_ps, c_ts, c_hs;
+  long long num_pages, page_size;
+  const int* page_table;
+  long long table_ld, max_pages;
+  const int* cu_q;
+  const int* kv_lens;
+  long long batch, tokens, max_q, max_kv;
+  int heads, kv_heads, head_dim;
+  float scale;
+  void* out;
+  long long o_ts, o_hs;
+  float* lse;
+  void* workspace;
+  int out_f32, bf16;
+};
+
+// few rows per sequence and key head (paged_decode.cu): at most 16
+bool paged_is_decode(const PagedArgs& a);
+long long paged_decode_workspace(const PagedArgs& a);
+int paged_decode(const PagedArgs& a, cudaStream_t stream);
+
 // test probe of the bounded waits (probe.cu)
 int wait_timeout_probe(const void* src, long long limit_ns, int* out, cudaStream_t stream);
 

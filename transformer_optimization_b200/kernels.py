@@ -8,6 +8,7 @@ tensor on the CPU, a wrong dtype or a missing library raises.
 
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -402,6 +403,158 @@ def attn_merge(o_acc: torch.Tensor, lse_acc: torch.Tensor, o_part: torch.Tensor,
     bs16 = out16.stride(0) if out16 is not None else 0
     _abi.call("tf_attn_merge", _ptr(o_acc), _ptr(lse_acc), _ptr(o_part), _ptr(lse_part), o_acc.stride(1),
               o_acc.stride(0), _ptr(out16), ld16, bs16, bsz, heads, sq, dq // heads, _stream())
+
+
+# ------------------------------------------------- serving: positions and cache
+# The wrappers below check shapes, types and strides before they look for a
+# device, so a malformed call is refused the same way on any host; they run on
+# the tensors' own device and that device's current stream.
+
+
+def _launch_device(name: str, *ts: Optional[torch.Tensor]) -> torch.device:
+    _need_cuda(name, *ts)
+    devices = {t.device for t in ts if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"{name}: operands are on different devices {sorted(map(str, devices))}")
+    return devices.pop()
+
+
+def _need_index(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, n: Optional[int]) -> None:
+    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
+        size = "" if n is None else f" with {n} entries"
+        raise ValueError(f"{name}: {what} must be contiguous {str(dtype).split('.')[-1]}{size}")
+
+
+def _need_heads(name: str, what: str, t: torch.Tensor, dtype: torch.dtype) -> None:
+    if t.dtype != dtype or t.dim() != 3 or t.stride(-1) != 1:
+        raise ValueError(f"{name}: {what} must be [tokens, heads, head_dim] {str(dtype).split('.')[-1]} with unit inner "
+                         "stride")
+
+
+def _need_cache(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, hd: int) -> None:
+    for t in (k_cache, v_cache):
+        if t.dtype != like.dtype or t.dim() != 4 or t.stride(-1) != 1 or t.shape[3] != hd:
+            raise ValueError(f"{name}: k_cache and v_cache must be [pages, page_size, kv_heads, {hd}] of the queries' "
+                             "type with unit inner stride")
+    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+        raise ValueError(f"{name}: k_cache and v_cache must have matching shapes and strides")
+
+
+def rotary_freqs(rot: int, base: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
+                 trained_len: int = 4096, device=None) -> Tuple[torch.Tensor, float]:
+    """Angles per position of `rotary`, fp64 [rot / 2], and its mscale.
+
+    f_i = base^(-2i / rot). scaling (contexts `factor` times the trained
+    length): "linear" f_i / factor; "ntk" base * factor^(rot / (rot - 2)), which
+    keeps f_0 and divides the last f by factor; "parts" keeps the f_i that turn 32 times or more
+    within trained_len, divides those that turn once or less by factor, and
+    blends in between, with mscale = 0.1 ln(factor) + 1."""
+    if rot < 2 or rot % 2:
+        raise ValueError(f"rotary_freqs: rot={rot} must be even and positive")
+    if scaling not in ("none", "linear", "ntk", "parts"):
+        raise ValueError(f"rotary_freqs: scaling {scaling!r} (none, linear, ntk or parts)")
+    if not (base > 0 and factor >= 1 and trained_len > 0):
+        raise ValueError("rotary_freqs: base and trained_len must be positive, factor at least 1")
+    if scaling == "ntk" and rot > 2:
+        base = base * factor ** (rot / (rot - 2))
+    f = base ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    mscale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "parts":
+        keep = ((trained_len * f / (2 * math.pi) - 1) / 31).clamp(0, 1)
+        f = f * keep + f / factor * (1 - keep)
+        mscale = 0.1 * math.log(factor) + 1
+    return f.to(device), mscale
+
+
+def _rotary_operands(name, q, k, positions, freqs):
+    if q.dtype not in HALF_TYPES:
+        raise ValueError(f"{name}: q must be fp16 or bf16")
+    _need_heads(name, "q", q, q.dtype)
+    if k is not None:
+        _need_heads(name, "k", k, q.dtype)
+        if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+            raise ValueError(f"{name}: q and k must have the same tokens and head_dim")
+    _need_index(name, "positions", positions, torch.int64, q.shape[0])
+    _need_index(name, "freqs", freqs, torch.float64, None)
+    rot = 2 * freqs.numel()
+    if not 2 <= rot <= q.shape[2]:
+        raise ValueError(f"{name}: {freqs.numel()} frequencies turn {rot} elements of a head of {q.shape[2]}")
+    return rot
+
+
+def _rotary_out(name, what, x, out):
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _need_heads(name, what, out, x.dtype)
+    if out.shape != x.shape:
+        raise ValueError(f"{name}: {what} must have its input's shape")
+    return out
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, *,
+           interleaved: bool = False, mscale: float = 1.0, q_out: Optional[torch.Tensor] = None,
+           k_out: Optional[torch.Tensor] = None):
+    """Rotary positions (tf_rotary): the first 2 * len(freqs) elements of every
+    head are turned in pairs by positions[t] * freqs[i] and scaled by mscale,
+    the rest copied.
+
+    q [T, H, hd], k [T, KVH, hd] or None: fp16 or bf16 views with unit inner
+    stride (head slices of a packed QKV buffer); positions int64 [T] (any
+    sign); freqs fp64 (rotary_freqs). Pairs are (i, i + rot/2), or
+    (2i, 2i + 1) with interleaved. q_out / k_out may be q / k (in place) but
+    must not overlap them otherwise. The transpose, and so the gradient, is
+    rotary at -positions. Returns (q_out, k_out)."""
+    rot = _rotary_operands("rotary", q, k, positions, freqs)
+    q_out = _rotary_out("rotary", "q_out", q, q_out)
+    if k is not None:
+        k_out = _rotary_out("rotary", "k_out", k, k_out)
+    elif k_out is not None:
+        raise ValueError("rotary: k_out without k")
+    dev = _launch_device("rotary", q, k, positions, freqs, q_out, k_out)
+    t, h, hd = q.shape
+    flags = (_abi.TF_ROTARY_INTERLEAVED if interleaved else 0) | (_abi.TF_ROTARY_BF16 if q.dtype == torch.bfloat16 else 0)
+    ks, kos = (k.stride()[:2], k_out.stride()[:2]) if k is not None else ((0, 0), (0, 0))
+    with torch.cuda.device(dev):
+        _abi.call("tf_rotary", _ptr(q), q.stride(0), q.stride(1), _ptr(q_out), q_out.stride(0), q_out.stride(1),
+                  _ptr(k), *ks, _ptr(k_out), *kos, _ptr(positions), _ptr(freqs), t, h,
+                  k.shape[1] if k is not None else 0, hd, rot, float(mscale), flags, _stream())
+    return q_out, k_out
+
+
+def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor,
+                  k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, *, interleaved: bool = False,
+                  mscale: float = 1.0, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`rotary` whose turned keys, and the values, go into a paged cache
+    (tf_rotary_append): token t's to row slots[t] % page_size of page
+    slots[t] // page_size.
+
+    k_cache, v_cache [pages, page_size, KVH, hd] of q's type, unit inner
+    stride (another order of the middle axes is a transposed view); slots int64
+    [T], distinct where not negative. A negative slot writes nothing (a padding
+    token); one past the cache writes nothing and sets the device status
+    (108). Returns q_out."""
+    name = "rotary_append"
+    rot = _rotary_operands(name, q, k, positions, freqs)
+    _need_heads(name, "v", v, q.dtype)
+    if v.shape != k.shape:
+        raise ValueError(f"{name}: v must have k's shape")
+    _need_cache(name, k_cache, v_cache, q, q.shape[2])
+    if k_cache.shape[2] != k.shape[1] or k_cache.shape[1] < 1:
+        raise ValueError(f"{name}: the cache holds {k_cache.shape[2]} key heads, k has {k.shape[1]}")
+    _need_index(name, "slots", slots, torch.int64, q.shape[0])
+    q_out = _rotary_out(name, "q_out", q, q_out)
+    dev = _launch_device(name, q, k, v, positions, freqs, k_cache, v_cache, slots, q_out)
+    t, h, hd = q.shape
+    flags = (_abi.TF_ROTARY_INTERLEAVED if interleaved else 0) | (_abi.TF_ROTARY_BF16 if q.dtype == torch.bfloat16 else 0)
+    with torch.cuda.device(dev):
+        _abi.call("tf_rotary_append", _ptr(q), q.stride(0), q.stride(1), _ptr(q_out), q_out.stride(0),
+                  q_out.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1),
+                  _ptr(positions), _ptr(freqs), _ptr(k_cache), _ptr(v_cache), *k_cache.stride()[:3],
+                  k_cache.shape[0], k_cache.shape[1], _ptr(slots), t, h, k.shape[1], hd, rot, float(mscale), flags,
+                  _stream())
+    return q_out
 
 
 def wait_timeout_probe(src: torch.Tensor, limit_ns: int) -> torch.Tensor:
