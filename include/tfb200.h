@@ -318,6 +318,57 @@ int tf_rotary_append(const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int
                      int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rot, float mscale,
                      int flags, void* stream);
 
+/* Flash attention of sequences of different lengths laid end to end, with
+ * grouped heads:
+ *   out_i = sum_j softmax_j(scale * q_i . k_j) v_j   over the keys of i's own sequence
+ * q [tokens, heads, head_dim] (token and head strides q_ts, q_hs, unit inner
+ * stride; fp16, bf16 with TF_ATTN_BF16), k and v [k_tokens, kv_heads,
+ * head_dim]; query head h reads key head h / (heads / kv_heads). Sequence b
+ * has queries cu_q[b] .. cu_q[b+1]-1 and keys cu_k[b] .. cu_k[b+1]-1 (int32
+ * [batch + 1], ascending). With TF_ATTN_CAUSAL query i of a sequence sees keys
+ * 0 .. i + (keys - queries): its last query stands at its last key. out: q's
+ * type (fp32 with TF_ATTN_OUT_F32); lse: fp32 [heads, tokens] natural
+ * log-sum-exp or NULL. A query without admissible keys gets out = 0 and
+ * lse = -inf; rows of out and lse outside the sequences are left as they were.
+ * Keys and values of other sequences never reach a result, whatever they hold
+ * (a non-finite value of the own sequence reaches the rows of its 128-row tile
+ * even where the causal mask hides it). max_q, max_k: host bounds on a
+ * sequence's queries and keys (max_k only sizes the key split). Lengths or
+ * offsets outside the arrays, or queries past max_q, are cut to the bound and
+ * set device code 108. head_dim 64 or 128; heads a multiple of kv_heads, at
+ * most 128 times; scale > 0; bases 16-byte aligned, strides multiples of 8.
+ * workspace: tf_flash_packed_workspace bytes (the same sizes, tokens = q's
+ * rows), 16-byte aligned; calls that overlap in time need their own.
+ * Replaces the attention of the reference's fp16 path for ragged batches,
+ * which it runs padded under a key mask (torch_transformer_benchmark.py:
+ * 4146-4161). */
+int64_t tf_flash_packed_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                  int64_t max_q, int64_t max_k);
+int tf_flash_packed(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
+                    const void* v, int64_t v_ts, int64_t v_hs, const int32_t* cu_q, const int32_t* cu_k, void* out,
+                    int64_t o_ts, int64_t o_hs, float* lse, int64_t tokens, int64_t k_tokens, int64_t batch,
+                    int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_q, int64_t max_k, float scale,
+                    int flags, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The same over a paged cache: key j of sequence b is row j % page_size of
+ * page page_table[b * table_ld + j / page_size] (int32, max_pages per
+ * sequence) of k_cache / v_cache [num_pages, page_size, kv_heads, head_dim]
+ * (page, token and head strides c_ps, c_ts, c_hs, unit inner stride); it has
+ * kv_lens[b] keys (int32 [batch]), its new tokens' among them. Table entries
+ * past a sequence's last page are not read, nor the rest of that page. A page
+ * outside the cache reads as zeros and sets device code 108. page_size: a
+ * power of two from 16. Up to 16 / (heads / kv_heads) new tokens per sequence
+ * (max_q) take a streaming kernel that splits the keys over all SMs. No
+ * reference counterpart: the reference keeps no cache. */
+int64_t tf_flash_paged_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                 int64_t max_q, int64_t max_k);
+int tf_flash_paged(const void* q, int64_t q_ts, int64_t q_hs, const void* k_cache, const void* v_cache, int64_t c_ps,
+                   int64_t c_ts, int64_t c_hs, int64_t num_pages, int64_t page_size, const int32_t* page_table,
+                   int64_t table_ld, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_lens, void* out,
+                   int64_t o_ts, int64_t o_hs, float* lse, int64_t tokens, int64_t batch, int64_t heads,
+                   int64_t kv_heads, int64_t head_dim, int64_t max_q, int64_t max_k, float scale, int flags,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -76,6 +76,12 @@ SIGNATURES = {
                    _I64, _I64, _I64, _I64, _I64, _F, _I, _P], _I),
     "tf_rotary_append": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P,
                           _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _F, _I, _P], _I),
+    "tf_flash_packed_workspace": ([_I64, _I64, _I64, _I64, _I64, _I64, _I64], _I64),
+    "tf_flash_paged_workspace": ([_I64, _I64, _I64, _I64, _I64, _I64, _I64], _I64),
+    "tf_flash_packed": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _P,
+                         _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _P, _I64, _P], _I),
+    "tf_flash_paged": ([_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64,
+                        _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _P, _I64, _P], _I),
     "tf_attn_merge": ([_P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P], _I),
     "tf_gemm_splitk_workspace": ([_I64, _I64, _I64, _I], _I64),
     "tf_gemm_splitk": ([_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _P, _I64, _P], _I),

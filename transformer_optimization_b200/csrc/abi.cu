@@ -120,7 +120,7 @@ static int encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t
                   const cuuint32_t* box) {
   auto fn = encode_fn();
   if (fn == nullptr) return set_error(TF_ERR_DRIVER, "cuTensorMapEncodeTiled entry point unavailable");
-  cuuint32_t elem[3] = {1, 1, 1};
+  cuuint32_t elem[4] = {1, 1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), dims, strides, box, elem,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -146,6 +146,25 @@ int make_tmap_3d_f16(CUtensorMap* map, const void* base, long long inner, long l
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * 2), static_cast<cuuint64_t>(bstride * 2)};
   cuuint32_t box[3] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_rows), 1};
   return encode(map, 3, base, dims, strides, box);
+}
+
+int make_tmap_4d_f16(CUtensorMap* map, const void* base, const long long (&dims)[4], const long long (&pitch)[3],
+                     const int (&box)[4]) {
+  if (!aligned16(base)) return set_error(TF_ERR_ALIGN, "tensor map: base alignment");
+  cuuint64_t d[4], st[3];
+  cuuint32_t bx[4];
+  for (int i = 0; i < 4; ++i) {
+    d[i] = static_cast<cuuint64_t>(dims[i] > 0 ? dims[i] : 1);
+    bx[i] = static_cast<cuuint32_t>(box[i]);
+  }
+  for (int i = 0; i < 3; ++i) {
+    // the pitch of an axis of one entry is never used; any valid value stands in
+    const long long bytes = dims[i + 1] > 1 ? pitch[i] * 2 : 16;
+    if (bytes <= 0 || bytes % 16 != 0 || bytes >= (1ll << 40))
+      return set_error(TF_ERR_ALIGN, "tensor map: pitch of %lld elements", pitch[i]);
+    st[i] = static_cast<cuuint64_t>(bytes);
+  }
+  return encode(map, 4, base, d, st, bx);
 }
 
 }  // namespace tfb
@@ -595,6 +614,127 @@ int tf_rotary_append(const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int
   a.tokens = tokens;
   a.mscale = mscale;
   return rotary_common("tf_rotary_append", a, heads, kv_heads, head_dim, rot, flags, stream);
+}
+
+static int seq_common(const char* fn, tfb::SeqArgs& a, int64_t heads, int64_t kv_heads, int64_t head_dim, int flags,
+                      void* stream) {
+  clear_message();
+  if (flags & ~(TF_ATTN_CAUSAL | TF_ATTN_OUT_F32 | TF_ATTN_BF16)) return set_error(TF_ERR_SHAPE, "%s: unknown flags", fn);
+  int rc = narrow_dims(fn, heads, kv_heads, head_dim, 0);
+  if (rc) return rc;
+  a.heads = static_cast<int>(heads);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.head_dim = static_cast<int>(head_dim);
+  a.causal = (flags & TF_ATTN_CAUSAL) != 0;
+  a.out_f32 = (flags & TF_ATTN_OUT_F32) != 0;
+  a.bf16 = (flags & TF_ATTN_BF16) != 0;
+  rc = tfb::seq_check(a, fn);
+  if (rc) return rc;
+  rc = begin_call();
+  if (rc) return rc;
+  return tfb::seq_attention(a, as_stream(stream));
+}
+
+static int64_t seq_workspace_common(const char* fn, int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads,
+                                    int64_t head_dim, int64_t max_q, int64_t max_k, int64_t page_size) {
+  clear_message();
+  if (narrow_dims(fn, heads, kv_heads, head_dim, 0)) return -1;
+  tfb::SeqArgs a = {};
+  a.tokens = tokens;
+  a.batch = batch;
+  a.heads = static_cast<int>(heads);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.head_dim = static_cast<int>(head_dim);
+  a.max_q = max_q;
+  a.max_k = max_k;
+  a.page_size = page_size;
+  a.scale = 1.f;
+  a.q = a.k = a.v = &a;  // sizes only: the pointer checks see an aligned stand-in
+  a.out = &a;
+  a.cu_q = a.cu_k = a.kv_lens = reinterpret_cast<const int*>(&a);
+  if (tfb::seq_check(a, fn)) return -1;
+  if (begin_call()) return -1;
+  return tfb::seq_workspace(a);
+}
+
+int64_t tf_flash_packed_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                  int64_t max_q, int64_t max_k) {
+  return seq_workspace_common("tf_flash_packed_workspace", tokens, batch, heads, kv_heads, head_dim, max_q, max_k, 0);
+}
+
+int64_t tf_flash_paged_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                 int64_t max_q, int64_t max_k) {
+  return seq_workspace_common("tf_flash_paged_workspace", tokens, batch, heads, kv_heads, head_dim, max_q, max_k, 16);
+}
+
+int tf_flash_packed(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
+                    const void* v, int64_t v_ts, int64_t v_hs, const int32_t* cu_q, const int32_t* cu_k, void* out,
+                    int64_t o_ts, int64_t o_hs, float* lse, int64_t tokens, int64_t k_tokens, int64_t batch,
+                    int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_q, int64_t max_k, float scale,
+                    int flags, void* workspace, int64_t workspace_bytes, void* stream) {
+  tfb::SeqArgs a = {};
+  a.q = q;
+  a.q_ts = q_ts;
+  a.q_hs = q_hs;
+  a.k = k;
+  a.k_ts = k_ts;
+  a.k_hs = k_hs;
+  a.v = v;
+  a.v_ts = v_ts;
+  a.v_hs = v_hs;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.out = out;
+  a.o_ts = o_ts;
+  a.o_hs = o_hs;
+  a.lse = lse;
+  a.tokens = tokens;
+  a.k_tokens = k_tokens;
+  a.batch = batch;
+  a.max_q = max_q;
+  a.max_k = max_k;
+  a.scale = scale;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  return seq_common("tf_flash_packed", a, heads, kv_heads, head_dim, flags, stream);
+}
+
+int tf_flash_paged(const void* q, int64_t q_ts, int64_t q_hs, const void* k_cache, const void* v_cache, int64_t c_ps,
+                   int64_t c_ts, int64_t c_hs, int64_t num_pages, int64_t page_size, const int32_t* page_table,
+                   int64_t table_ld, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_lens, void* out,
+                   int64_t o_ts, int64_t o_hs, float* lse, int64_t tokens, int64_t batch, int64_t heads,
+                   int64_t kv_heads, int64_t head_dim, int64_t max_q, int64_t max_k, float scale, int flags,
+                   void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_message();
+  if (page_size <= 0) return set_error(TF_ERR_SHAPE, "tf_flash_paged: page_size=%lld", static_cast<long long>(page_size));
+  tfb::SeqArgs a = {};
+  a.q = q;
+  a.q_ts = q_ts;
+  a.q_hs = q_hs;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.k_ps = a.v_ps = c_ps;
+  a.k_ts = a.v_ts = c_ts;
+  a.k_hs = a.v_hs = c_hs;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.page_table = page_table;
+  a.table_ld = table_ld;
+  a.max_pages = max_pages;
+  a.cu_q = cu_q;
+  a.kv_lens = kv_lens;
+  a.out = out;
+  a.o_ts = o_ts;
+  a.o_hs = o_hs;
+  a.lse = lse;
+  a.tokens = tokens;
+  a.batch = batch;
+  a.max_q = max_q;
+  a.max_k = max_k;
+  a.scale = scale;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  return seq_common("tf_flash_paged", a, heads, kv_heads, head_dim, flags, stream);
 }
 
 }  // extern "C"

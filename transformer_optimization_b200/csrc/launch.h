@@ -41,6 +41,11 @@ int make_tmap_2d_f16(CUtensorMap* map, const void* base, long long inner, long l
 int make_tmap_3d_f16(CUtensorMap* map, const void* base, long long inner, long long rows, long long batches,
                      long long ld, long long bstride, int box_inner, int box_rows);
 
+// 4-D fp16 tensor map, 128-byte swizzle: extents `dims` (inner first), pitches
+// of the outer three axes in elements, box `box`.
+int make_tmap_4d_f16(CUtensorMap* map, const void* base, const long long (&dims)[4], const long long (&pitch)[3],
+                     const int (&box)[4]);
+
 // Programmatic dependent launch. Every kernel of this library is launched
 // with programmatic stream serialization: it may start (barrier set-up,
 // TMEM allocation, tensor-map prefetch) while the previous kernel on the
@@ -175,32 +180,43 @@ struct RotaryArgs {
 int rotary_check(const RotaryArgs& a, const char* fn);
 int rotary(const RotaryArgs& a, cudaStream_t stream);
 
-// attention of new tokens over a paged cache
-struct PagedArgs {
-  const void* q;
+// Attention of sequences of different lengths: keys and values packed end to
+// end (page_table null) or in a paged cache.
+struct SeqArgs {
+  const void* q;  // [tokens, heads, head_dim]
   long long q_ts, q_hs;
-  const void* k_cache;
-  const void* v_cache;
-  long long c_ps, c_ts, c_hs;
-  long long num_pages, page_size;
-  const int* page_table;
+  const void* k;  // packed: [k_tokens, kv_heads, head_dim]; paged: [num_pages, page_size, kv_heads, head_dim]
+  const void* v;
+  long long k_ps, k_ts, k_hs;  // page (paged), token and head pitches of keys and of values
+  long long v_ps, v_ts, v_hs;
+  long long num_pages, page_size;  // paged
+  const int* page_table;           // paged: [batch, max_pages] with pitch table_ld
   long long table_ld, max_pages;
-  const int* cu_q;
-  const int* kv_lens;
-  long long batch, tokens, max_q, max_kv;
+  const int* cu_q;    // [batch + 1] first query token of each sequence
+  const int* cu_k;    // packed: the same of the keys
+  const int* kv_lens; // paged: [batch] keys of each sequence
+  long long batch, tokens, k_tokens, max_q, max_k;
   int heads, kv_heads, head_dim;
   float scale;
-  void* out;
+  void* out;  // [tokens, heads, head_dim]
   long long o_ts, o_hs;
-  float* lse;
+  float* lse;  // [heads, tokens] or null
   void* workspace;
-  int out_f32, bf16;
+  long long workspace_bytes;
+  int causal, out_f32, bf16;
 };
 
-// few rows per sequence and key head (paged_decode.cu): at most 16
-bool paged_is_decode(const PagedArgs& a);
-long long paged_decode_workspace(const PagedArgs& a);
-int paged_decode(const PagedArgs& a, cudaStream_t stream);
+// Argument checks that need no device (the C entries make them first).
+int seq_check(const SeqArgs& a, const char* fn);
+// bytes of workspace a call with these sizes needs (0: none)
+long long seq_workspace(const SeqArgs& a);
+int seq_attention(const SeqArgs& a, cudaStream_t stream);
+
+// the paged form for at most 16 query rows per sequence and key head
+// (paged_decode.cu); seq_attention dispatches to it
+bool paged_is_decode(const SeqArgs& a);
+long long paged_decode_workspace(const SeqArgs& a);
+int paged_decode(const SeqArgs& a, cudaStream_t stream);
 
 // test probe of the bounded waits (probe.cu)
 int wait_timeout_probe(const void* src, long long limit_ns, int* out, cudaStream_t stream);

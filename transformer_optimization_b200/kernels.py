@@ -411,33 +411,49 @@ def attn_merge(o_acc: torch.Tensor, lse_acc: torch.Tensor, o_part: torch.Tensor,
 # the tensors' own device and that device's current stream.
 
 
-def _launch_device(name: str, *ts: Optional[torch.Tensor]) -> torch.device:
-    _need_cuda(name, *ts)
-    devices = {t.device for t in ts if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"{name}: operands are on different devices {sorted(map(str, devices))}")
-    return devices.pop()
+def _device_of(name: str, first: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
+    """The index of the CUDA device that holds every operand."""
+    dev = first.get_device()
+    if dev < 0:
+        _need_cuda(name, first)
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            _need_cuda(name, t)
+            raise ValueError(f"{name}: operands are on different devices (cuda:{dev} and {t.device})")
+    return dev
+
+
+def _launch(dev: int, fn: str, *args) -> None:
+    """Call an ABI function on device `dev` and its current stream (the
+    stream is looked up by index and the device is switched only when it is
+    not the current one: together they cost a small call a third of its
+    host time otherwise)."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch._C._cuda_getDevice():
+        _abi.call(fn, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            _abi.call(fn, *args, stream)
 
 
 def _need_index(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, n: Optional[int]) -> None:
-    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
+    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
         size = "" if n is None else f" with {n} entries"
         raise ValueError(f"{name}: {what} must be contiguous {str(dtype).split('.')[-1]}{size}")
 
 
 def _need_heads(name: str, what: str, t: torch.Tensor, dtype: torch.dtype) -> None:
-    if t.dtype != dtype or t.dim() != 3 or t.stride(-1) != 1:
+    if t.dtype != dtype or t.dim() != 3 or t.stride()[2] != 1:
         raise ValueError(f"{name}: {what} must be [tokens, heads, head_dim] {str(dtype).split('.')[-1]} with unit inner "
                          "stride")
 
 
 def _need_cache(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, hd: int) -> None:
-    for t in (k_cache, v_cache):
-        if t.dtype != like.dtype or t.dim() != 4 or t.stride(-1) != 1 or t.shape[3] != hd:
-            raise ValueError(f"{name}: k_cache and v_cache must be [pages, page_size, kv_heads, {hd}] of the queries' "
-                             "type with unit inner stride")
-    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
-        raise ValueError(f"{name}: k_cache and v_cache must have matching shapes and strides")
+    if k_cache.dtype != like.dtype or k_cache.dim() != 4 or k_cache.stride()[3] != 1 or k_cache.shape[3] != hd:
+        raise ValueError(f"{name}: k_cache and v_cache must be [pages, page_size, kv_heads, {hd}] of the queries' "
+                         "type with unit inner stride")
+    if v_cache.dtype != k_cache.dtype or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+        raise ValueError(f"{name}: k_cache and v_cache must have one type and matching shapes and strides")
 
 
 def rotary_freqs(rot: int, base: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
@@ -512,14 +528,13 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         k_out = _rotary_out("rotary", "k_out", k, k_out)
     elif k_out is not None:
         raise ValueError("rotary: k_out without k")
-    dev = _launch_device("rotary", q, k, positions, freqs, q_out, k_out)
+    dev = _device_of("rotary", q, k, positions, freqs, q_out, k_out)
     t, h, hd = q.shape
     flags = (_abi.TF_ROTARY_INTERLEAVED if interleaved else 0) | (_abi.TF_ROTARY_BF16 if q.dtype == torch.bfloat16 else 0)
     ks, kos = (k.stride()[:2], k_out.stride()[:2]) if k is not None else ((0, 0), (0, 0))
-    with torch.cuda.device(dev):
-        _abi.call("tf_rotary", _ptr(q), q.stride(0), q.stride(1), _ptr(q_out), q_out.stride(0), q_out.stride(1),
-                  _ptr(k), *ks, _ptr(k_out), *kos, _ptr(positions), _ptr(freqs), t, h,
-                  k.shape[1] if k is not None else 0, hd, rot, float(mscale), flags, _stream())
+    _launch(dev, "tf_rotary", q.data_ptr(), *q.stride()[:2], q_out.data_ptr(), *q_out.stride()[:2], _ptr(k), *ks,
+            _ptr(k_out), *kos, positions.data_ptr(), freqs.data_ptr(), t, h, k.shape[1] if k is not None else 0, hd, rot,
+            mscale, flags)
     return q_out, k_out
 
 
@@ -545,16 +560,148 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
         raise ValueError(f"{name}: the cache holds {k_cache.shape[2]} key heads, k has {k.shape[1]}")
     _need_index(name, "slots", slots, torch.int64, q.shape[0])
     q_out = _rotary_out(name, "q_out", q, q_out)
-    dev = _launch_device(name, q, k, v, positions, freqs, k_cache, v_cache, slots, q_out)
+    dev = _device_of(name, q, k, v, positions, freqs, k_cache, v_cache, slots, q_out)
     t, h, hd = q.shape
     flags = (_abi.TF_ROTARY_INTERLEAVED if interleaved else 0) | (_abi.TF_ROTARY_BF16 if q.dtype == torch.bfloat16 else 0)
-    with torch.cuda.device(dev):
-        _abi.call("tf_rotary_append", _ptr(q), q.stride(0), q.stride(1), _ptr(q_out), q_out.stride(0),
-                  q_out.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1),
-                  _ptr(positions), _ptr(freqs), _ptr(k_cache), _ptr(v_cache), *k_cache.stride()[:3],
-                  k_cache.shape[0], k_cache.shape[1], _ptr(slots), t, h, k.shape[1], hd, rot, float(mscale), flags,
-                  _stream())
+    _launch(dev, "tf_rotary_append", q.data_ptr(), *q.stride()[:2], q_out.data_ptr(), *q_out.stride()[:2], k.data_ptr(),
+            *k.stride()[:2], v.data_ptr(), *v.stride()[:2], positions.data_ptr(), freqs.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), *k_cache.stride()[:3], *k_cache.shape[:2], slots.data_ptr(), t, h, k.shape[1], hd, rot,
+            mscale, flags)
     return q_out
+
+
+def _seq_operands(name, q, kv_heads, cu_q, max_q, scale, out, out_dtype, lse, want_lse):
+    if q.dtype not in HALF_TYPES:
+        raise ValueError(f"{name}: q must be fp16 or bf16")
+    t, h, hd = q.shape
+    if hd not in (64, 128):
+        raise ValueError(f"{name}: head_dim {hd} (64 or 128)")
+    if kv_heads < 1 or h % kv_heads or not 1 <= h // kv_heads <= 128:
+        raise ValueError(f"{name}: {h} query heads over {kv_heads} key heads")
+    _need_index(name, "cu_q", cu_q, torch.int32, None)
+    if cu_q.shape[0] < 1 or max_q < 0:
+        raise ValueError(f"{name}: cu_q must hold batch + 1 offsets and max_q must not be negative")
+    if not 0 < scale < math.inf:
+        raise ValueError(f"{name}: scale must be positive and finite")
+    if out_dtype is None:
+        out_dtype = q.dtype if out is None else out.dtype
+    if out_dtype not in (q.dtype, torch.float32):
+        raise ValueError(f"{name}: out_dtype must be q's type or fp32")
+    if out is None:
+        out = torch.empty(t, h, hd, dtype=out_dtype, device=q.device)
+    else:
+        _need_heads(name, "out", out, out_dtype)
+        if out.shape != q.shape:
+            raise ValueError(f"{name}: out must have q's shape")
+    if lse is None:
+        if want_lse:
+            lse = torch.empty(h, t, dtype=torch.float32, device=q.device)
+    elif lse.dtype != torch.float32 or lse.shape != (h, t) or not lse.is_contiguous():
+        raise ValueError(f"{name}: lse must be contiguous fp32 [heads, tokens]")
+    flags = (_abi.TF_ATTN_OUT_F32 if out_dtype == torch.float32 else 0) | (
+        _abi.TF_ATTN_BF16 if q.dtype == torch.bfloat16 else 0)
+    return out, lse, flags
+
+
+def _seq_workspace(name, fn, dev, workspace, *sizes):
+    if dev == torch._C._cuda_getDevice():
+        need = _abi.call_value(fn, *sizes)
+    else:
+        with torch.cuda.device(dev):
+            need = _abi.call_value(fn, *sizes)
+    if workspace is None:
+        if need == 0:
+            return None, 0
+        return torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev)), need
+    if not workspace.is_contiguous() or workspace.get_device() != dev:
+        raise ValueError(f"{name}: workspace must be contiguous, on the operands' device")
+    size = workspace.numel() * workspace.element_size()
+    if size < need:
+        raise ValueError(f"{name}: workspace of {need} bytes needed")
+    return workspace, size
+
+
+def flash_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                           max_q: int, scale: float, *, max_k: Optional[int] = None, causal: bool = False,
+                           out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                           lse: Optional[torch.Tensor] = None, want_lse: bool = False,
+                           workspace: Optional[torch.Tensor] = None):
+    """Flash attention of sequences of different lengths laid end to end, with
+    grouped heads (tf_flash_packed).
+
+    q [T, H, hd], k and v [Tk, KVH, hd]: fp16 or bf16 views with unit inner
+    stride (head slices of a packed QKV buffer); query head h reads key head
+    h // (H // KVH). Sequence b has queries cu_q[b]:cu_q[b + 1] and keys
+    cu_k[b]:cu_k[b + 1] (int32 [B + 1]); max_q and max_k bound their lengths
+    (max_k, Tk if None, only decides how far the keys are split). causal:
+    query i sees keys up to i + (keys - queries). Returns (out [T, H, hd], lse
+    fp32 [H, T] or None); rows outside the sequences are left as they were, a
+    query without keys gets 0 and -inf. With out_dtype fp32 the results of
+    key ranges merge by attn_merge (a batch of one). workspace (allocated if
+    None) must not serve two calls at a time."""
+    name = "flash_attention_packed"
+    _need_heads(name, "q", q, q.dtype)
+    _need_heads(name, "k", k, q.dtype)
+    _need_heads(name, "v", v, q.dtype)
+    if k.shape != v.shape or k.shape[2] != q.shape[2]:
+        raise ValueError(f"{name}: k and v must have one shape and q's head_dim")
+    out, lse, flags = _seq_operands(name, q, k.shape[1], cu_q, max_q, scale, out, out_dtype, lse, want_lse)
+    _need_index(name, "cu_k", cu_k, torch.int32, cu_q.shape[0])
+    if max_k is None:
+        max_k = k.shape[0]
+    elif max_k < 0:
+        raise ValueError(f"{name}: max_k must not be negative")
+    dev = _device_of(name, q, k, v, cu_q, cu_k, out, lse)
+    (t, h, hd), (tk, g, _), b = q.shape, k.shape, cu_q.shape[0] - 1
+    ws, ws_bytes = _seq_workspace(name, "tf_flash_packed_workspace", dev, workspace, t, b, h, g, hd, max_q, max_k)
+    _launch(dev, "tf_flash_packed", q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
+            *v.stride()[:2], cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), *out.stride()[:2], _ptr(lse), t, tk, b, h,
+            g, hd, max_q, max_k, scale, flags | (_abi.TF_ATTN_CAUSAL if causal else 0), _ptr(ws), ws_bytes)
+    return out, lse
+
+
+def flash_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                          cu_q: torch.Tensor, kv_lens: torch.Tensor, max_q: int, scale: float, *,
+                          max_kv: Optional[int] = None, causal: bool = True, out: Optional[torch.Tensor] = None,
+                          out_dtype: Optional[torch.dtype] = None, lse: Optional[torch.Tensor] = None,
+                          want_lse: bool = False, workspace: Optional[torch.Tensor] = None):
+    """Flash attention of each sequence's new tokens (one, a few, or a chunk)
+    over its paged cache (tf_flash_paged).
+
+    q [T, H, hd] as in flash_attention_packed, sequence b's new tokens
+    cu_q[b]:cu_q[b + 1], at most max_q; k_cache, v_cache [pages, page_size, KVH,
+    hd] (page_size a power of two from 16; another order of the middle axes is
+    a transposed view); page_table int32 [B, max_pages], kv_lens int32 [B]: the
+    keys of sequence b, its new tokens' (rotary_append) among them, are the
+    first kv_lens[b] rows of its pages. Table entries past the last page are
+    not read. max_kv bounds kv_lens (the table's capacity if None; it only
+    decides how far the keys are split). Returns (out, lse) as
+    flash_attention_packed."""
+    name = "flash_attention_paged"
+    _need_heads(name, "q", q, q.dtype)
+    _need_cache(name, k_cache, v_cache, q, q.shape[2])
+    pages, page, g = k_cache.shape[:3]
+    if page < 16 or page & (page - 1):
+        raise ValueError(f"{name}: page_size {page} (a power of two from 16)")
+    out, lse, flags = _seq_operands(name, q, g, cu_q, max_q, scale, out, out_dtype, lse, want_lse)
+    b = cu_q.shape[0] - 1
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != b or (
+            page_table.shape[1] > 1 and page_table.stride()[1] != 1):
+        raise ValueError(f"{name}: page_table must be int32 [{b}, max_pages] with unit inner stride")
+    _need_index(name, "kv_lens", kv_lens, torch.int32, b)
+    max_pages = page_table.shape[1]
+    if max_kv is None:
+        max_kv = max_pages * page
+    elif max_kv < 0:
+        raise ValueError(f"{name}: max_kv must not be negative")
+    dev = _device_of(name, q, k_cache, v_cache, page_table, cu_q, kv_lens, out, lse)
+    t, h, hd = q.shape
+    ws, ws_bytes = _seq_workspace(name, "tf_flash_paged_workspace", dev, workspace, t, b, h, g, hd, max_q, max_kv)
+    _launch(dev, "tf_flash_paged", q.data_ptr(), *q.stride()[:2], k_cache.data_ptr(), v_cache.data_ptr(),
+            *k_cache.stride()[:3], pages, page, page_table.data_ptr(), page_table.stride()[0], max_pages,
+            cu_q.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), *out.stride()[:2], _ptr(lse), t, b, h, g, hd, max_q,
+            max_kv, scale, flags | (_abi.TF_ATTN_CAUSAL if causal else 0), _ptr(ws), ws_bytes)
+    return out, lse
 
 
 def wait_timeout_probe(src: torch.Tensor, limit_ns: int) -> torch.Tensor:
