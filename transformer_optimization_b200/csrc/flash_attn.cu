@@ -75,8 +75,8 @@ struct AttnCfg {
   static constexpr int kVOff = kKOff + kKStages * kTileBytes;
   static constexpr int kBarOff = kVOff + kVStages * kTileBytes;
   // q_full, k_full/empty[KS], v_full/empty[VS], s_full[NS],
-  // p_full[2 tiles x 2 alternating], o_full[2], turn[2], drain[2], pv_done[NS]
-  static constexpr int kNumBars = 1 + 2 * kKStages + 2 * kVStages + kNS + 4 + 2 + 2 + 2 + kNS;
+  // p_full[2 tiles x 2 alternating], turn[2], drain[2], pv_done[NS]
+  static constexpr int kNumBars = 1 + 2 * kKStages + 2 * kVStages + kNS + 4 + 2 + 2 + kNS;
   static constexpr int kBytes = kBarOff + kNumBars * 8 + 16;
   static constexpr int kAlloc = kBytes + 1024;
   // TMEM columns: S/P slots at 0, 128, ..; O_t at kNS*128 + t*HD (512 in all)
@@ -152,8 +152,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   constexpr int NS = C::kNS;
   uint64_t* s_full = v_empty + VS;
   uint64_t* p_full = s_full + NS;  // [tile * 2 + (block & 1)]: alternating, so no waiter falls two phases behind
-  uint64_t* o_full = p_full + 4;   // [tile]: every PV of the tile so far has landed in O
-  uint64_t* turn = o_full + 2;     // exp-phase hand-off between the two softmax warpgroups
+  uint64_t* turn = p_full + 4;     // exp-phase hand-off between the two softmax warpgroups
   uint64_t* drain = turn + 2;       // [issuer]: end-of-kernel drain of each MMA issuer
   uint64_t* pv_done = drain + 2;    // [slot]: the PV that read this slot's P has completed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + NS);
@@ -202,7 +201,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int i = 0; i < NS; ++i) mbar_init(&s_full[i], 1);
     for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 128);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&o_full[i], 1);
       mbar_init(&turn[i], 128);
     }
     mbar_init(&drain[0], 1);
@@ -322,7 +320,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             umma_f16_ts(tmem_base + C::kTmO + t * HD, tmem_base + C::kTmS + slot * 128 + k * 8,
                         smem_desc_sw128(va + k * 2048, 16384, 1024), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
           umma_commit(&pv_done[slot]);
-          umma_commit(&o_full[t]);
           if (last_user(t, j)) umma_commit(&v_empty[j % VS]);
         }
       }
@@ -348,12 +345,23 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const int n_pp = nmin;  // blocks where both tiles take turns
     const float c = p.scale_log2;
 
+    // issue order of (t, j)
+    auto pair_at = [&](int j) { return j < nmin ? 2 * j + t : 2 * nmin + (j - nmin); };
+    // every PV up to the tile's block j has landed in O. The slot's barrier is
+    // exact: S of this thread's newest pair waited for the PV NS pairs back,
+    // so no phase before the awaited one of that slot is open. (One barrier
+    // per tile would not do: with one tile alone its PVs run up to NS behind.)
+    auto wait_pv = [&](int j) {
+      const int q = pair_at(j);
+      return mbar_wait(&pv_done[q % NS], (q / NS) & 1, p.status, kDevTimeoutSoftmax);
+    };
+
     float m_ref = -INFINITY;  // reference max (scaled log2 domain)
     float l = 0.f;            // row sum
     bool ok = true;
 
     for (int j = 0; j < nb; ++j) {
-      const int q = j < nmin ? 2 * j + t : 2 * nmin + (j - nmin);  // issue order of (t, j)
+      const int q = pair_at(j);
       const int slot = q % NS;
       if (!(ok = mbar_wait(&s_full[slot], (q / NS) & 1, p.status, kDevTimeoutSoftmax))) break;
       tc_fence_after();
@@ -436,7 +444,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const float m_new = fmaxf(m_ref, m_row);
         const float alpha = m_ref == -INFINITY ? 0.f : ex2_f32(m_ref - m_new);
         // every PV so far (the last is block j-1) must have landed in O
-        if (!(ok = mbar_wait(&o_full[t], (j - 1) & 1, p.status, kDevTimeoutSoftmax))) break;
+        if (!(ok = wait_pv(j - 1))) break;
         tc_fence_after();
         rescale_o<HD>(tm_o, alpha);
         l *= alpha;
@@ -504,7 +512,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       float inv = 0.f;
       uint32_t ov[HD];
       if (nb > 0) {
-        if (!(ok = mbar_wait(&o_full[t], (nb - 1) & 1, p.status, kDevTimeoutSoftmax))) {
+        if (!(ok = wait_pv(nb - 1))) {
           // fall through to the barrier; nothing is written
         } else {
           tc_fence_after();
