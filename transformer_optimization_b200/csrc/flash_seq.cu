@@ -684,7 +684,7 @@ int seq_check(const SeqArgs& a, const char* fn) {
                      a.heads, a.kv_heads);
   const long long most = 1ll << 30;
   if (a.batch < 0 || a.batch > most || a.tokens < 0 || a.tokens > most || a.k_tokens < 0 || a.k_tokens > most ||
-      a.max_q < 0 || a.max_k < 0)
+      a.max_q < 0 || a.max_k < 0 || a.batch * a.kv_heads > most)
     return set_error(TF_ERR_SHAPE, "%s: sizes out of range", fn);
   if (!(a.scale > 0.f) || !(a.scale - a.scale == 0.f))
     return set_error(TF_ERR_SHAPE, "%s: scale must be positive and finite", fn);

@@ -38,6 +38,7 @@ constexpr int kDecTile = 16;                        // keys per warp and step
 constexpr int kDecUnit = kDecWarps * kDecTile;      // keys per unit
 constexpr int kDecRows = 16;                        // query rows per item
 constexpr int kDecCtasPerSm = 2;
+constexpr int kSeqCache = 32;  // sequences of a block's run whose lengths are kept in shared memory
 
 struct DecodeK {
   SeqArgs a;
@@ -55,7 +56,9 @@ struct DecCfg {
   static constexpr int kTileBytes = kDecTile * HD * 2;             // K or V tile
   static constexpr int kRing = kDecWarps * kStages * 2 * kTileBytes;  // 96 KB
   static constexpr int kMerge = 2 * kDecRows * HD * 4;              // two warps' O
-  static constexpr int kBytes = kRing + kMerge;
+  static constexpr int kStat = 2 * kDecWarps * kDecRows * 4;         // the warps' row maxima and sums
+  static constexpr int kBytes = kRing + kMerge + kStat + kSeqCache * 12;
+  static_assert(kDecCtasPerSm * (kBytes + 1024) <= 228 * 1024, "two blocks per SM");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
@@ -107,21 +110,29 @@ __device__ __forceinline__ SeqLens decode_lens(const SeqArgs& a, int group, int 
   const long long cap = static_cast<long long>(a.max_pages) << page_shift;
   s.q0 = min(max(c0, 0), static_cast<int>(a.tokens));
   s.q = min(max(c1, s.q0), static_cast<int>(a.tokens)) - s.q0;
-  s.q = min(s.q, kDecRows / group);
+  s.q = min(s.q, min(kDecRows / group, static_cast<int>(a.max_q)));
   s.k = kv < 0 ? 0 : (kv > cap ? static_cast<int>(cap) : kv);
   s.bad = c0 < 0 || c1 < c0 || c1 > a.tokens || s.q != c1 - c0 || s.k != kv;
   return s;
 }
 __device__ __forceinline__ int units_of(const SeqLens& s) { return s.q > 0 ? (s.k + kDecUnit - 1) / kDecUnit : 0; }
 
-// Sum over all sequences of units, and (optionally) the sequence that holds
-// unit number `at` when every sequence's units count kv_heads times: `seq`
-// and the number of units before it. One warp.
-__device__ __forceinline__ long long find_unit(const DecodeK& p, long long at, int& seq, long long& before) {
+// Units of all sequences (every key head counted), one warp; four sequences
+// per lane are requested at a time.
+__device__ __forceinline__ long long total_units(const DecodeK& p) {
+  long long n = 0;
+#pragma unroll 4
+  for (int b = lane_id(); b < p.a.batch; b += 32)
+    n += units_of(decode_lens(p.a, p.group, p.page_shift, b));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+  return n * p.a.kv_heads;
+}
+
+// The sequence that holds unit `at`, and the number of units before it.
+__device__ __forceinline__ int find_unit(const DecodeK& p, long long at, long long& before) {
   const int lane = lane_id();
   long long run = 0;
-  seq = -1;
-  before = 0;
   for (int base = 0; base < p.a.batch; base += 32) {
     const int b = base + lane;
     long long n = 0;
@@ -133,19 +144,28 @@ __device__ __forceinline__ long long find_unit(const DecodeK& p, long long at, i
       if (lane >= d) inc += up;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, run + inc > at);
-    if (seq < 0 && hit != 0) {
+    if (hit != 0) {
       const int l = __ffs(hit) - 1;
-      seq = base + l;
       before = run + __shfl_sync(0xffffffffu, inc - n, l);
+      return base + l;
     }
     run += __shfl_sync(0xffffffffu, inc, 31);
   }
-  return run;
+  before = run;
+  return -1;
 }
 
-__device__ __forceinline__ long long run_start(long long total, int block, int blocks) {
-  return total * block / blocks;
-}
+// Block c's run of units: total / blocks each, one more for the first
+// total % blocks.
+struct Runs {
+  long long per, extra;
+  __device__ __forceinline__ Runs(long long total, int blocks) : per(total / blocks), extra(total % blocks) {}
+  __device__ __forceinline__ long long start(long long c) const { return c * per + (c < extra ? c : extra); }
+  __device__ __forceinline__ int block_of(long long u) const {
+    const long long head = extra * (per + 1);
+    return static_cast<int>(u < head ? u / (per + 1) : extra + (u - head) / per);
+  }
+};
 
 template <int HD, int DT>
 __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_kernel(const DecodeK p) {
@@ -153,41 +173,119 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_ke
   constexpr int KT = HD / 16;       // k-steps of Q K^T
   constexpr int CH = HD / 8;        // 16-byte chunks per tile row
   constexpr int RPI = 32 / CH;      // tile rows one warp-wide copy covers
-  extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ float s_m[kDecWarps][kDecRows], s_l[kDecWarps][kDecRows];
+  extern __shared__ __align__(128) uint8_t smem[];
   const int lane = lane_id();
   const int warp = warp_id();
   const SeqArgs& a = p.a;
   const uint32_t ring = smem_u32(smem) + warp * (C::kStages * 2 * C::kTileBytes);
   float* s_o = reinterpret_cast<float*>(smem + C::kRing);
+  auto s_m = reinterpret_cast<float(*)[kDecRows]>(smem + C::kRing + C::kMerge);
+  auto s_l = s_m + kDecWarps;
+  auto s_seq = reinterpret_cast<int(*)[3]>(smem + C::kRing + C::kMerge + C::kStat);
   pdl_wait();
   pdl_trigger();
 
-  int seq;
+  const Runs runs(total_units(p), gridDim.x);
+  const long long u_begin = runs.start(blockIdx.x);
+  const int steps = static_cast<int>(runs.start(blockIdx.x + 1) - u_begin);
+  if (steps == 0) return;
   long long before;
-  long long total = find_unit(p, -1, seq, before);
-  const long long u_end = run_start(total, blockIdx.x + 1, gridDim.x);
-  long long u = run_start(total, blockIdx.x, gridDim.x);
-  if (u >= u_end) return;
-  find_unit(p, u, seq, before);
+  const int seq0 = find_unit(p, u_begin, before);
+  for (int i = threadIdx.x; i < kSeqCache; i += kDecWarps * 32) {
+    SeqLens s = {};
+    if (seq0 + i < a.batch) s = decode_lens(a, p.group, p.page_shift, seq0 + i);
+    s_seq[i][0] = s.q0;
+    s_seq[i][1] = s.q;
+    s_seq[i][2] = s.k;
+  }
+  __syncthreads();
 
-  bool first_segment = true;
-  while (u < u_end) {
-    // ---- the item (sequence, key head) and this run's part of it
-    SeqLens s = decode_lens(a, p.group, p.page_shift, seq);
-    int nu = units_of(s);
-    while (nu == 0 || u - before >= static_cast<long long>(nu) * a.kv_heads) {
-      before += static_cast<long long>(nu) * a.kv_heads;
-      s = decode_lens(a, p.group, p.page_shift, ++seq);
-      nu = units_of(s);
+  // A position in the run: unit c of the nu units of (seq, kvh). Loads run
+  // kStages - 1 units ahead of the products with a position of their own, so
+  // the ring stays full across items.
+  struct At {
+    int seq, kvh, c, nu;
+    SeqLens s;
+  };
+  auto enter = [&](At& x, int seq) {  // the first sequence from `seq` on that has units
+    while (true) {
+      if (seq - seq0 < kSeqCache) {
+        const int* e = s_seq[seq - seq0];
+        x.s.q0 = e[0];
+        x.s.q = e[1];
+        x.s.k = e[2];
+      } else {
+        x.s = decode_lens(a, p.group, p.page_shift, seq);
+      }
+      x.nu = units_of(x.s);
+      if (x.nu > 0) break;
+      ++seq;
     }
-    const int kvh = static_cast<int>((u - before) / nu);
-    const int c_begin = static_cast<int>(u - before - static_cast<long long>(kvh) * nu);  // first unit of the segment
-    const int c_end = static_cast<int>(u_end - u < nu - c_begin ? c_begin + (u_end - u) : nu);
-    const bool whole = c_begin == 0 && c_end == nu;
+    x.seq = seq;
+  };
+  auto advance = [&](At& x, bool more) {  // to the next unit of the run
+    if (++x.c < x.nu || !more) return;
+    x.c = 0;
+    if (++x.kvh == a.kv_heads) {
+      x.kvh = 0;
+      enter(x, x.seq + 1);
+    }
+  };
+  At now, ahead;
+  enter(now, seq0);
+  now.kvh = static_cast<int>((u_begin - before) / now.nu);
+  now.c = static_cast<int>(u_begin - before - static_cast<long long>(now.kvh) * now.nu);
+  ahead = now;
+
+  // this warp's tile of a unit lies within one page: its table entry, and its copy
+  auto page_of = [&](const At& x) {
+    const int key0 = x.c * kDecUnit + warp * kDecTile;
+    return key0 < x.s.k ? a.page_table[x.seq * a.table_ld + (key0 >> p.page_shift)] : 0;
+  };
+  auto issue = [&](const At& x, int page, int stage) {
+    const int key0 = x.c * kDecUnit + warp * kDecTile;
+    const uint32_t dst = ring + stage * (2 * C::kTileBytes);
+    const bool ok = page >= 0 && page < a.num_pages;
+    if (!ok && lane == 0) record_error(p.status, kDevBadIndex);
+    const int row = key0 & ((1 << p.page_shift) - 1);
+    const int ch = lane % CH;
+    const long long pg = ok ? page : 0;
+    const uint16_t* kp = static_cast<const uint16_t*>(a.k) + pg * a.k_ps + x.kvh * a.k_hs + row * a.k_ts + ch * 8;
+    const uint16_t* vp = static_cast<const uint16_t*>(a.v) + pg * a.v_ps + x.kvh * a.v_hs + row * a.v_ts + ch * 8;
+#pragma unroll
+    for (int i = 0; i < kDecTile / RPI; ++i) {
+      const int r = i * RPI + lane / CH;
+      const bool on = ok && key0 + r < x.s.k;
+      const uint32_t d = dst + r * (HD * 2) + ((ch ^ (r & 7)) << 4);
+      cp_async16(d, on ? kp + r * a.k_ts : static_cast<const uint16_t*>(a.k), on);
+      cp_async16(d + C::kTileBytes, on ? vp + r * a.v_ts : static_cast<const uint16_t*>(a.v), on);
+    }
+  };
+  int loaded = 0;  // units issued
+  int page = page_of(ahead);
+  auto load_next = [&](int stage) {
+    if (loaded < steps) {
+      if (ahead.c * kDecUnit + warp * kDecTile < ahead.s.k) issue(ahead, page, stage);
+      ++loaded;
+      advance(ahead, loaded < steps);
+      if (loaded < steps) page = page_of(ahead);
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < C::kStages - 1; ++i) load_next(i);
+
+  int stage = 0, free_stage = C::kStages - 1;
+  bool first_segment = true;
+  for (int step = 0; step < steps;) {
+    // ---- a segment: this run's part of one item
+    const SeqLens s = now.s;
+    const int kvh = now.kvh;
+    const int c_end = min(now.nu, now.c + steps - step);
+    const bool whole = now.c == 0 && c_end == now.nu;
     const int rows = s.q * p.group;
 
-    // ---- queries as mma operands: rows lane/4 and lane/4 + 8
+    // queries as mma operands: rows lane/4 and lane/4 + 8
     uint32_t qf[KT][4];
     {
       const int r0 = lane >> 2, r1 = r0 + 8;
@@ -209,36 +307,6 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_ke
     const int lim0 = a.causal ? s.k - s.q + (lane >> 2) / p.group + 1 : s.k;
     const int lim1 = a.causal ? s.k - s.q + ((lane >> 2) + 8) / p.group + 1 : s.k;
 
-    const int* table = a.page_table + static_cast<long long>(seq) * a.table_ld;
-    const uint16_t* kbase = static_cast<const uint16_t*>(a.k) + static_cast<long long>(kvh) * a.k_hs;
-    const uint16_t* vbase = static_cast<const uint16_t*>(a.v) + static_cast<long long>(kvh) * a.v_hs;
-    auto page_of = [&](int c) {  // page of this warp's tile of unit c (a tile lies within a page)
-      const int key0 = c * kDecUnit + warp * kDecTile;
-      return c < c_end && key0 < s.k ? __ldg(table + (key0 >> p.page_shift)) : 0;
-    };
-    auto issue = [&](int c, int page) {
-      if (c < c_end) {
-        const int key0 = c * kDecUnit + warp * kDecTile;
-        const int stage = (c - c_begin) % C::kStages;
-        const uint32_t dst = ring + stage * (2 * C::kTileBytes);
-        const bool ok = page >= 0 && page < a.num_pages;
-        if (!ok && key0 < s.k && lane == 0) record_error(p.status, kDevBadIndex);
-        const int row = key0 & ((1 << p.page_shift) - 1);
-        const uint16_t* kp = kbase + static_cast<long long>(ok ? page : 0) * a.k_ps + row * a.k_ts;
-        const uint16_t* vp = vbase + static_cast<long long>(ok ? page : 0) * a.v_ps + row * a.v_ts;
-        const int ch = lane % CH;
-#pragma unroll
-        for (int i = 0; i < kDecTile / RPI; ++i) {
-          const int r = i * RPI + lane / CH;
-          const bool on = ok && key0 + r < s.k;
-          const uint32_t d = dst + r * (HD * 2) + ((ch ^ (r & 7)) << 4);
-          cp_async16(d, on ? kp + r * a.k_ts + ch * 8 : kbase, on);
-          cp_async16(d + C::kTileBytes, on ? vp + r * a.v_ts + ch * 8 : vbase, on);
-        }
-      }
-      cp_commit();
-    };
-
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     float o[HD / 8][4];
 #pragma unroll
@@ -246,22 +314,13 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_ke
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
 
-    int ahead[C::kStages];
-#pragma unroll
-    for (int i = 0; i < C::kStages; ++i) ahead[i] = page_of(c_begin + i);
-#pragma unroll
-    for (int i = 0; i < C::kStages - 1; ++i) issue(c_begin + i, ahead[i]);
-    int page = ahead[C::kStages - 1];
-    for (int c = c_begin; c < c_end; ++c) {
+    for (int c = now.c; c < c_end; ++c, ++step) {
       cp_wait<C::kStages - 2>();
       __syncwarp();
+      load_next(free_stage);  // the stage of the unit before this one
       const int key0 = c * kDecUnit + warp * kDecTile;
-      // the stage of the tile before this one is free: refill it first, with
-      // the page read one step ago
-      issue(c + C::kStages - 1, page);
-      page = page_of(c + C::kStages);
       if (key0 < s.k) {
-        const uint32_t kt = ring + ((c - c_begin) % C::kStages) * (2 * C::kTileBytes);
+        const uint32_t kt = ring + stage * (2 * C::kTileBytes);
         const uint32_t vt = kt + C::kTileBytes;
         // S = Q K^T: two 8-key column tiles; matrices (keys 0-7 | 8-15) x (k 0-7 | 8-15)
         float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
@@ -337,9 +396,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_ke
           }
         }
       }
+      free_stage = stage;
+      stage = stage + 1 == C::kStages ? 0 : stage + 1;
     }
-    cp_wait<0>();
-    __syncwarp();
 
     // ---- join the four warps: common maximum, then O summed in warp order
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
@@ -434,90 +493,95 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_ke
         }
       }
     }
-    u += c_end - c_begin;
+    // on to the next item (or to the end)
     first_segment = false;
+    now.c = c_end - 1;
+    advance(now, step < steps);
   }
+  cp_wait<0>();
 }
 
 // Joins the partial results of every item that more than one block worked on,
 // and writes the rows of sequences without keys (out 0, log-sum-exp -inf).
-// One block per (sequence, key head).
+// One block per (sequence, key head) and row; its warps take every fourth
+// partial result, so that long joins are not a chain of memory latencies, and
+// add up in warp order.
 template <int HD, int DT>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const DecodeK p, int blocks) {
+__global__ void __launch_bounds__(kDecWarps * 32) paged_combine_kernel(const DecodeK p, int blocks) {
+  constexpr int E = HD / 32;
+  __shared__ float s_o[kDecWarps][HD];
+  __shared__ float s_l[kDecWarps];
   const SeqArgs& a = p.a;
   pdl_wait();
   pdl_trigger();
-  const int seq = blockIdx.x, kvh = blockIdx.y;
+  const int seq = blockIdx.x / a.kv_heads, kvh = blockIdx.x - seq * a.kv_heads;
+  const int r = blockIdx.y;
   const int lane = lane_id(), warp = warp_id();
   const SeqLens s = decode_lens(a, p.group, p.page_shift, seq);
-  const int rows = s.q * p.group;
-  if (s.bad && kvh == 0 && threadIdx.x == 0) record_error(p.status, kDevBadIndex);
-  if (rows == 0) return;
+  if (s.bad && kvh == 0 && r == 0 && threadIdx.x == 0) record_error(p.status, kDevBadIndex);
+  if (r >= s.q * p.group) return;
   const int nu = units_of(s);
-  long long run = 0, before = 0;  // units of all sequences, and of those before this one
-  for (int base = 0; base < a.batch; base += 32) {
-    const int b = base + lane;
-    long long n = 0;
-    if (b < a.batch) n = static_cast<long long>(units_of(decode_lens(a, p.group, p.page_shift, b))) * a.kv_heads;
-    long long mine = b < seq ? n : 0;
+  int c0 = 0, c1 = -1;
+  long long ua = 0;
+  Runs runs(0, 1);
+  if (nu > 0) {
+    long long all = 0, mine = 0;  // units of all sequences, and of those before this one
+#pragma unroll 4
+    for (int b = lane; b < a.batch; b += 32) {
+      const int n = units_of(decode_lens(a, p.group, p.page_shift, b));
+      all += n;
+      mine += b < seq ? n : 0;
+    }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) {
-      n += __shfl_xor_sync(0xffffffffu, n, d);
+      all += __shfl_xor_sync(0xffffffffu, all, d);
       mine += __shfl_xor_sync(0xffffffffu, mine, d);
     }
-    run += n;
-    before += mine;
-  }
-  const long long ua = before + static_cast<long long>(kvh) * nu, ub = ua + nu;
-  // blocks whose runs meet [ua, ub): run_start(c) <= ua < run_start(c + 1)
-  int c0 = 0, c1 = -1;
-  if (nu > 0) {
-    c0 = static_cast<int>(ua * blocks / run);
-    while (c0 + 1 < blocks && run_start(run, c0 + 1, blocks) <= ua) ++c0;
-    while (run_start(run, c0, blocks) > ua) --c0;
-    c1 = static_cast<int>((ub - 1) * blocks / run);
-    while (c1 + 1 < blocks && run_start(run, c1 + 1, blocks) <= ub - 1) ++c1;
-    while (run_start(run, c1, blocks) > ub - 1) --c1;
+    runs = Runs(all * a.kv_heads, blocks);
+    ua = mine * a.kv_heads + static_cast<long long>(kvh) * nu;
+    c0 = runs.block_of(ua);
+    c1 = runs.block_of(ua + nu - 1);
     if (c0 == c1) return;  // one block saw all of it and wrote the result
   }
-  for (int r = warp; r < rows; r += 4) {
-    float m = -INFINITY;
-    for (int c = c0; c <= c1; ++c) {
-      if (run_start(run, c, blocks) == run_start(run, c + 1, blocks)) continue;  // an empty run wrote nothing
-      const long long part = 2ll * c + (run_start(run, c, blocks) >= ua ? 0 : 1);
-      m = fmaxf(m, p.l_part[part * kDecRows + r]);
-    }
-    float l = 0.f, acc[HD / 32];
+  // partial result of block c: its first segment's place, unless the block
+  // began with an earlier item (only c0 can have)
+  const bool late = runs.start(c0) < ua;
+  auto part = [&](int c) { return 2ll * c + (late && c == c0 ? 1 : 0); };
+  float m = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.l_part[part(c) * kDecRows + r]);
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) acc[i] = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      if (run_start(run, c, blocks) == run_start(run, c + 1, blocks)) continue;
-      const long long part = 2ll * c + (run_start(run, c, blocks) >= ua ? 0 : 1);
-      const float lg = p.l_part[part * kDecRows + r];
-      if (lg == -INFINITY) continue;
-      const float w = ex2_f32(lg - m);
-      l += w;
-      const float* src = p.o_part + (part * kDecRows + r) * HD + lane * (HD / 32);
+  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  float l = 0.f, acc[E];
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) acc[i] = fmaf(w, src[i], acc[i]);
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int tok = s.q0 + r / p.group, head = kvh * p.group + r % p.group;
-    const long long base =
-        static_cast<long long>(tok) * a.o_ts + static_cast<long long>(head) * a.o_hs + lane * (HD / 32);
+  for (int i = 0; i < E; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += kDecWarps) {
+    const float lg = p.l_part[part(c) * kDecRows + r];
+    const float w = lg == -INFINITY ? 0.f : ex2_f32(lg - m);
+    const float* src = p.o_part + (part(c) * kDecRows + r) * HD + lane * E;
+    l += w;
 #pragma unroll
-    for (int i = 0; i < HD / 32; i += 2) {
-      if (a.out_f32) {
-        *reinterpret_cast<float2*>(static_cast<float*>(a.out) + base + i) = make_float2(acc[i] * inv, acc[i + 1] * inv);
-      } else {
-        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + base + i) =
-            pack2<DT>(acc[i] * inv, acc[i + 1] * inv);
-      }
-    }
-    if (a.lse != nullptr && lane == 0)
-      a.lse[static_cast<long long>(head) * a.tokens + tok] =
-          l > 0.f ? (m + __log2f(l)) * 0.69314718055994531f : -INFINITY;
+    for (int i = 0; i < E; ++i) acc[i] = fmaf(w, src[i], acc[i]);
   }
+#pragma unroll
+  for (int i = 0; i < E; ++i) s_o[warp][lane * E + i] = acc[i];
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const int tok = s.q0 + r / p.group, head = kvh * p.group + r % p.group;
+  const long long base = static_cast<long long>(tok) * a.o_ts + static_cast<long long>(head) * a.o_hs;
+  for (int i = threadIdx.x; i < HD; i += kDecWarps * 32) {
+    const float x = ((s_o[0][i] + s_o[1][i]) + (s_o[2][i] + s_o[3][i])) * inv;
+    if (a.out_f32) {
+      static_cast<float*>(a.out)[base + i] = x;
+    } else {
+      static_cast<uint16_t*>(a.out)[base + i] = static_cast<uint16_t>(pack2<DT>(x, 0.f) & 0xffffu);
+    }
+  }
+  if (a.lse != nullptr && threadIdx.x == 0)
+    a.lse[static_cast<long long>(head) * a.tokens + tok] =
+        l > 0.f ? (m + __log2f(l)) * 0.69314718055994531f : -INFINITY;
 }
 
 // Blocks of a call: every SM's share, but no more than there can be units.
@@ -541,7 +605,9 @@ int launch_decode(const DecodeK& k, int blocks, cudaStream_t stream) {
   }
   cudaError_t e = launch_k(kern, dim3(blocks), dim3(kDecWarps * 32), C::kBytes, stream, k);
   if (e == cudaSuccess)
-    e = launch_k(paged_combine_kernel<HD, DT>, dim3(k.a.batch, k.a.kv_heads), dim3(128), 0, stream, k, blocks);
+    e = launch_k(paged_combine_kernel<HD, DT>,
+                 dim3(static_cast<unsigned>(k.a.batch * k.a.kv_heads), static_cast<unsigned>(k.a.max_q * k.group)),
+                 dim3(kDecWarps * 32), 0, stream, k, blocks);
   if (e != cudaSuccess) return set_error(TF_ERR_LAUNCH, "paged decode launch: %s", cudaGetErrorString(e));
   return TF_OK;
 }
