@@ -8,23 +8,25 @@
 // Bound by HBM: every key and value is read once for all of the group's
 // query heads, 4 * rows flop per element, far below the tensor rate. So the
 // kernel is a streaming kernel: each warp keeps a ring of 16-key tiles of its
-// own in shared memory (cp.async, no block barrier in the loop), and the
-// products run on mma.sync m16n8k16, whose 16 rows fit the group and whose
-// result layout feeds the probabilities straight back as the next operand
-// (the tcgen05 form needs 128 rows and a TMEM round trip per tile).
+// own in shared memory, filled by TMA from the page that holds them (no block
+// barrier in the loop, no per-lane addresses), and the products run on
+// mma.sync m16n8k16, whose 16 rows fit the group and whose result layout feeds
+// the probabilities straight back as the next operand (the tcgen05 form needs
+// 128 rows and a TMEM round trip per tile).
 //
 // Work is split over keys, not over sequences: all (sequence, key head) items
-// are cut into units of 64 keys, numbered through, and each block takes an
-// equal run of units, so one 100 000-key sequence and 64 ragged ones both
-// fill the card. A run that covers an item writes its result; the one or two
-// items that it covers in part leave fp32 partial results, which
-// paged_combine_kernel joins in unit order (no atomics: the result does not
-// depend on timing). Nothing in the workspace outlives the call.
+// are cut into units of 64 keys, numbered through with kSegment more places
+// per item for its start and end, and each block takes an equal run of places,
+// so one 100 000-key sequence and 64 ragged ones both fill the card. A run
+// that covers an item writes its result; the one or two items that it covers
+// in part leave fp32 partial results, which paged_combine_kernel joins in unit
+// order (no atomics: the result does not depend on timing). Nothing in the
+// workspace outlives the call.
 //
 // Scores, maxima and sums are fp32; the probabilities are rounded to the
 // 16-bit operand type for the second product (the sum takes them unrounded),
-// as in flash_fwd_tcgen05. Keys past a sequence's end are never read: their
-// tile rows are zero-filled, so what an unused part of a page holds cannot
+// as in flash_fwd_tcgen05. The value rows of a tile past the sequence's end
+// are zeroed before the product, so what an unused part of a page holds cannot
 // reach a result.
 #include "attn_common.cuh"
 #include "common.cuh"
@@ -37,6 +39,7 @@ constexpr int kDecWarps = 4;
 constexpr int kDecTile = 16;                        // keys per warp and step
 constexpr int kDecUnit = kDecWarps * kDecTile;      // keys per unit
 constexpr int kDecRows = 16;                        // query rows per item
+constexpr int kSegment = 2;                         // an item's start and end cost about two units (place numbering)
 constexpr int kDecCtasPerSm = 2;
 constexpr int kSeqCache = 32;  // sequences of a block's run whose lengths are kept in shared memory
 
@@ -55,21 +58,11 @@ struct DecCfg {
   static constexpr int kStages = HD == 64 ? 6 : 3;
   static constexpr int kTileBytes = kDecTile * HD * 2;             // K or V tile
   static constexpr int kRing = kDecWarps * kStages * 2 * kTileBytes;  // 96 KB
-  static constexpr int kMerge = 2 * kDecRows * HD * 4;              // two warps' O
-  static constexpr int kStat = 2 * kDecWarps * kDecRows * 4;         // the warps' row maxima and sums
-  static constexpr int kBytes = kRing + kMerge + kStat + kSeqCache * 12;
+  static constexpr int kMerge = kDecWarps * 8 * HD * 4;              // the warps' O, 8 rows
+  static constexpr int kStat = 2 * kDecWarps * kDecRows * 4;         // their row maxima and sums
+  static constexpr int kBytes = kRing + kMerge + kStat + kSeqCache * 12 + kDecWarps * kStages * 8;
   static_assert(kDecCtasPerSm * (kBytes + 1024) <= 228 * 1024, "two blocks per SM");
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  const int n = on ? 16 : 0;  // 0: zero-filled, the source is not read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -116,31 +109,34 @@ __device__ __forceinline__ SeqLens decode_lens(const SeqArgs& a, int group, int 
   return s;
 }
 __device__ __forceinline__ int units_of(const SeqLens& s) { return s.q > 0 ? (s.k + kDecUnit - 1) / kDecUnit : 0; }
-
-// Units of all sequences (every key head counted), one warp; four sequences
-// per lane are requested at a time.
-__device__ __forceinline__ long long total_units(const DecodeK& p) {
-  long long n = 0;
-#pragma unroll 4
-  for (int b = lane_id(); b < p.a.batch; b += 32)
-    n += units_of(decode_lens(p.a, p.group, p.page_shift, b));
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
-  return n * p.a.kv_heads;
+// places of one key head: none without units
+__device__ __forceinline__ int places_of(const SeqLens& s) {
+  const int n = units_of(s);
+  return n > 0 ? n + kSegment : 0;
 }
 
-// The sequence that holds unit `at`, and the number of units before it.
-__device__ __forceinline__ int find_unit(const DecodeK& p, long long at, long long& before) {
+// Places of all sequences (every key head counted), one warp; `mine` is
+// sequence lane's. The host bounds the total below 2^31.
+__device__ __forceinline__ int total_places(const DecodeK& p, int mine) {
+  int n = mine;
+#pragma unroll 4
+  for (int b = lane_id() + 32; b < p.a.batch; b += 32) n += places_of(decode_lens(p.a, p.group, p.page_shift, b));
+  return __reduce_add_sync(0xffffffffu, n) * p.a.kv_heads;
+}
+
+// The sequence that holds place `at`, and the number of places before it.
+__device__ __forceinline__ int find_place(const DecodeK& p, int mine, int at, int& before) {
   const int lane = lane_id();
-  long long run = 0;
+  int run = 0;
   for (int base = 0; base < p.a.batch; base += 32) {
     const int b = base + lane;
-    long long n = 0;
-    if (b < p.a.batch) n = static_cast<long long>(units_of(decode_lens(p.a, p.group, p.page_shift, b))) * p.a.kv_heads;
-    long long inc = n;
+    int n = mine;
+    if (base > 0) n = b < p.a.batch ? places_of(decode_lens(p.a, p.group, p.page_shift, b)) : 0;
+    n *= p.a.kv_heads;
+    int inc = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, inc, d);
+      const int up = __shfl_up_sync(0xffffffffu, inc, d);
       if (lane >= d) inc += up;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, run + inc > at);
@@ -155,42 +151,49 @@ __device__ __forceinline__ int find_unit(const DecodeK& p, long long at, long lo
   return -1;
 }
 
-// Block c's run of units: total / blocks each, one more for the first
+// Block c's run of places: total / blocks each, one more for the first
 // total % blocks.
 struct Runs {
-  long long per, extra;
-  __device__ __forceinline__ Runs(long long total, int blocks) : per(total / blocks), extra(total % blocks) {}
-  __device__ __forceinline__ long long start(long long c) const { return c * per + (c < extra ? c : extra); }
-  __device__ __forceinline__ int block_of(long long u) const {
-    const long long head = extra * (per + 1);
-    return static_cast<int>(u < head ? u / (per + 1) : extra + (u - head) / per);
+  int per, extra;
+  __device__ __forceinline__ Runs(int total, int blocks) : per(total / blocks), extra(total - per * blocks) {}
+  __device__ __forceinline__ int start(int c) const { return c * per + min(c, extra); }
+  __device__ __forceinline__ int block_of(int u) const {
+    const int head = extra * (per + 1);
+    return u < head ? u / (per + 1) : extra + (u - head) / per;
   }
 };
 
 template <int HD, int DT>
-__global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_kernel(const DecodeK p) {
+__global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm)
+    paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                        const __grid_constant__ DecodeK p) {
   using C = DecCfg<HD>;
-  constexpr int KT = HD / 16;       // k-steps of Q K^T
-  constexpr int CH = HD / 8;        // 16-byte chunks per tile row
-  constexpr int RPI = 32 / CH;      // tile rows one warp-wide copy covers
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int KT = HD / 16;  // k-steps of Q K^T
+  constexpr int kStageBytes = 2 * C::kTileBytes;
+  extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = lane_id();
   const int warp = warp_id();
   const SeqArgs& a = p.a;
-  const uint32_t ring = smem_u32(smem) + warp * (C::kStages * 2 * C::kTileBytes);
+  uint8_t* ring = smem + warp * (C::kStages * kStageBytes);
   float* s_o = reinterpret_cast<float*>(smem + C::kRing);
   auto s_m = reinterpret_cast<float(*)[kDecRows]>(smem + C::kRing + C::kMerge);
   auto s_l = s_m + kDecWarps;
   auto s_seq = reinterpret_cast<int(*)[3]>(smem + C::kRing + C::kMerge + C::kStat);
+  uint64_t* full =
+      reinterpret_cast<uint64_t*>(smem + C::kRing + C::kMerge + C::kStat + kSeqCache * 12) + warp * C::kStages;
+  if (lane == 0) {
+    for (int i = 0; i < C::kStages; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+  }
   pdl_wait();
   pdl_trigger();
 
-  const Runs runs(total_units(p), gridDim.x);
-  const long long u_begin = runs.start(blockIdx.x);
-  const int steps = static_cast<int>(runs.start(blockIdx.x + 1) - u_begin);
-  if (steps == 0) return;
-  long long before;
-  const int seq0 = find_unit(p, u_begin, before);
+  const int mine = lane < a.batch ? places_of(decode_lens(a, p.group, p.page_shift, lane)) : 0;
+  const Runs runs(total_places(p, mine), gridDim.x);
+  const int u_begin = runs.start(blockIdx.x), u_end = runs.start(blockIdx.x + 1);
+  if (u_begin == u_end) return;
+  int before;
+  const int seq0 = find_place(p, mine, u_begin, before);
   for (int i = threadIdx.x; i < kSeqCache; i += kDecWarps * 32) {
     SeqLens s = {};
     if (seq0 + i < a.batch) s = decode_lens(a, p.group, p.page_shift, seq0 + i);
@@ -200,15 +203,16 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_ke
   }
   __syncthreads();
 
-  // A position in the run: unit c of the nu units of (seq, kvh). Loads run
-  // kStages - 1 units ahead of the products with a position of their own, so
-  // the ring stays full across items.
+  // A position in the run: unit c of the nu units of (seq, kvh), with `left`
+  // places of the run from it on. Loads run kStages - 1 units ahead of the
+  // products with a position of their own, so the ring stays full across items.
   struct At {
-    int seq, kvh, c, nu;
+    int seq, kvh, c, nu, left;
     SeqLens s;
   };
-  auto enter = [&](At& x, int seq) {  // the first sequence from `seq` on that has units
-    while (true) {
+  auto enter = [&](At& x, int seq) {  // the first sequence from `seq` on that has units, or none
+    x.nu = 0;
+    for (; seq < a.batch && x.nu == 0; ++seq) {
       if (seq - seq0 < kSeqCache) {
         const int* e = s_seq[seq - seq0];
         x.s.q0 = e[0];
@@ -218,94 +222,103 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_ke
         x.s = decode_lens(a, p.group, p.page_shift, seq);
       }
       x.nu = units_of(x.s);
-      if (x.nu > 0) break;
-      ++seq;
+      x.seq = seq;
     }
-    x.seq = seq;
+    if (x.nu == 0) x.left = 0;
   };
-  auto advance = [&](At& x, bool more) {  // to the next unit of the run
-    if (++x.c < x.nu || !more) return;
+  auto next_item = [&](At& x) {
     x.c = 0;
     if (++x.kvh == a.kv_heads) {
       x.kvh = 0;
       enter(x, x.seq + 1);
     }
   };
-  At now, ahead;
+  auto step = [&](At& x) {  // past one unit, over the item's end places if it was the last
+    --x.left;
+    if (++x.c == x.nu) {
+      x.left -= kSegment;
+      if (x.left > 0) next_item(x);
+    }
+  };
+  At now;
+  now.left = u_end - u_begin;
   enter(now, seq0);
-  now.kvh = static_cast<int>((u_begin - before) / now.nu);
-  now.c = static_cast<int>(u_begin - before - static_cast<long long>(now.kvh) * now.nu);
-  ahead = now;
+  {
+    const int places = now.nu + kSegment;
+    now.kvh = (u_begin - before) / places;
+    now.c = u_begin - before - now.kvh * places;
+    if (now.c >= now.nu) {  // the run begins in an item's end places
+      now.left -= places - now.c;
+      if (now.left > 0) next_item(now);
+    }
+  }
+  At ahead = now;
 
-  // this warp's tile of a unit lies within one page: its table entry, and its copy
+  // this warp's tile of a unit lies within one page: its table entry
   auto page_of = [&](const At& x) {
     const int key0 = x.c * kDecUnit + warp * kDecTile;
-    return key0 < x.s.k ? a.page_table[x.seq * a.table_ld + (key0 >> p.page_shift)] : 0;
+    return x.left > 0 && key0 < x.s.k ? a.page_table[x.seq * a.table_ld + (key0 >> p.page_shift)] : 0;
   };
-  auto issue = [&](const At& x, int page, int stage) {
-    const int key0 = x.c * kDecUnit + warp * kDecTile;
-    const uint32_t dst = ring + stage * (2 * C::kTileBytes);
-    const bool ok = page >= 0 && page < a.num_pages;
-    if (!ok && lane == 0) record_error(p.status, kDevBadIndex);
-    const int row = key0 & ((1 << p.page_shift) - 1);
-    const int ch = lane % CH;
-    const long long pg = ok ? page : 0;
-    const uint16_t* kp = static_cast<const uint16_t*>(a.k) + pg * a.k_ps + x.kvh * a.k_hs + row * a.k_ts + ch * 8;
-    const uint16_t* vp = static_cast<const uint16_t*>(a.v) + pg * a.v_ps + x.kvh * a.v_hs + row * a.v_ts + ch * 8;
-#pragma unroll
-    for (int i = 0; i < kDecTile / RPI; ++i) {
-      const int r = i * RPI + lane / CH;
-      const bool on = ok && key0 + r < x.s.k;
-      const uint32_t d = dst + r * (HD * 2) + ((ch ^ (r & 7)) << 4);
-      cp_async16(d, on ? kp + r * a.k_ts : static_cast<const uint16_t*>(a.k), on);
-      cp_async16(d + C::kTileBytes, on ? vp + r * a.v_ts : static_cast<const uint16_t*>(a.v), on);
-    }
-  };
-  int loaded = 0;  // units issued
   int page = page_of(ahead);
   auto load_next = [&](int stage) {
-    if (loaded < steps) {
-      if (ahead.c * kDecUnit + warp * kDecTile < ahead.s.k) issue(ahead, page, stage);
-      ++loaded;
-      advance(ahead, loaded < steps);
-      if (loaded < steps) page = page_of(ahead);
+    if (ahead.left <= 0) return;
+    const int key0 = ahead.c * kDecUnit + warp * kDecTile;
+    if (key0 < ahead.s.k && lane == 0) {
+      const bool ok = page >= 0 && page < a.num_pages;
+      if (!ok) record_error(p.status, kDevBadIndex);
+      const int z = ok ? page : (1 << 30);  // past every cache: zeros
+      const int row = key0 & ((1 << p.page_shift) - 1);
+      uint8_t* dst = ring + stage * kStageBytes;
+      mbar_arrive_expect_tx(&full[stage], kStageBytes);
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c) {
+        tma_load_4d(dst + c * 2048, &tmK, &full[stage], c * 64, ahead.kvh, row, z);
+        tma_load_4d(dst + C::kTileBytes + c * 2048, &tmV, &full[stage], c * 64, ahead.kvh, row, z);
+      }
     }
-    cp_commit();
+    step(ahead);
+    page = page_of(ahead);
   };
 #pragma unroll
   for (int i = 0; i < C::kStages - 1; ++i) load_next(i);
 
+  // queries as mma operands: rows lane/4 and lane/4 + 8
+  uint32_t qf[KT][4];
+  auto load_q = [&](const At& x) {
+    const int rows = x.s.q * p.group;
+    const int r0 = lane >> 2, r1 = r0 + 8;
+    const uint16_t* q = static_cast<const uint16_t*>(a.q);
+    const int i0 = r0 / p.group, i1 = r1 / p.group;
+    const uint16_t* p0 = q + static_cast<long long>(x.s.q0 + i0) * a.q_ts +
+                         static_cast<long long>(x.kvh * p.group + (r0 - i0 * p.group)) * a.q_hs + (lane & 3) * 2;
+    const uint16_t* p1 = q + static_cast<long long>(x.s.q0 + i1) * a.q_ts +
+                         static_cast<long long>(x.kvh * p.group + (r1 - i1 * p.group)) * a.q_hs + (lane & 3) * 2;
+#pragma unroll
+    for (int k = 0; k < KT; ++k) {
+      qf[k][0] = r0 < rows ? *reinterpret_cast<const uint32_t*>(p0 + k * 16) : 0u;
+      qf[k][1] = r1 < rows ? *reinterpret_cast<const uint32_t*>(p1 + k * 16) : 0u;
+      qf[k][2] = r0 < rows ? *reinterpret_cast<const uint32_t*>(p0 + k * 16 + 8) : 0u;
+      qf[k][3] = r1 < rows ? *reinterpret_cast<const uint32_t*>(p1 + k * 16 + 8) : 0u;
+    }
+  };
+  if (now.left > 0) load_q(now);
+
   int stage = 0, free_stage = C::kStages - 1;
-  bool first_segment = true;
-  for (int step = 0; step < steps;) {
+  uint32_t parity = 0;  // bit i: the phase of stage i that its next tile completes
+  while (now.left > 0) {
     // ---- a segment: this run's part of one item
     const SeqLens s = now.s;
     const int kvh = now.kvh;
-    const int c_end = min(now.nu, now.c + steps - step);
-    const bool whole = now.c == 0 && c_end == now.nu;
+    const int c_begin = now.c;
+    const int c_end = min(now.nu, now.c + now.left);
+    const bool whole = c_begin == 0 && c_end == now.nu;
+    // the item began before this run: its partial result takes the second place
+    const bool earlier = now.left != u_end - u_begin && c_begin == 0;
     const int rows = s.q * p.group;
-
-    // queries as mma operands: rows lane/4 and lane/4 + 8
-    uint32_t qf[KT][4];
-    {
-      const int r0 = lane >> 2, r1 = r0 + 8;
-      const uint16_t* q = static_cast<const uint16_t*>(a.q);
-      const int i0 = r0 / p.group, i1 = r1 / p.group;
-      const uint16_t* p0 = q + static_cast<long long>(s.q0 + i0) * a.q_ts +
-                           static_cast<long long>(kvh * p.group + (r0 - i0 * p.group)) * a.q_hs + (lane & 3) * 2;
-      const uint16_t* p1 = q + static_cast<long long>(s.q0 + i1) * a.q_ts +
-                           static_cast<long long>(kvh * p.group + (r1 - i1 * p.group)) * a.q_hs + (lane & 3) * 2;
-#pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        qf[k][0] = r0 < rows ? *reinterpret_cast<const uint32_t*>(p0 + k * 16) : 0u;
-        qf[k][1] = r1 < rows ? *reinterpret_cast<const uint32_t*>(p1 + k * 16) : 0u;
-        qf[k][2] = r0 < rows ? *reinterpret_cast<const uint32_t*>(p0 + k * 16 + 8) : 0u;
-        qf[k][3] = r1 < rows ? *reinterpret_cast<const uint32_t*>(p1 + k * 16 + 8) : 0u;
-      }
-    }
     // keys row r admits: up to its token's own position (causal)
     const int lim0 = a.causal ? s.k - s.q + (lane >> 2) / p.group + 1 : s.k;
     const int lim1 = a.causal ? s.k - s.q + ((lane >> 2) + 8) / p.group + 1 : s.k;
+    const int lim_min = a.causal ? s.k - s.q + 1 : s.k;
 
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     float o[HD / 8][4];
@@ -314,14 +327,26 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_ke
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
 
-    for (int c = now.c; c < c_end; ++c, ++step) {
-      cp_wait<C::kStages - 2>();
-      __syncwarp();
-      load_next(free_stage);  // the stage of the unit before this one
+    for (int c = c_begin; c < c_end; ++c) {
+      __syncwarp();           // every lane is done with the tile before this one:
+      load_next(free_stage);  // its stage is refilled
       const int key0 = c * kDecUnit + warp * kDecTile;
       if (key0 < s.k) {
-        const uint32_t kt = ring + stage * (2 * C::kTileBytes);
+        mbar_wait(&full[stage], (parity >> stage) & 1, p.status, kDevTimeoutProducer);
+        parity ^= 1u << stage;
+        uint8_t* tile = ring + stage * kStageBytes;
+        const uint32_t kt = smem_u32(tile);
         const uint32_t vt = kt + C::kTileBytes;
+        if (key0 + kDecTile > s.k) {
+          // the sequence ends inside the tile: zero the value rows behind it
+          const int valid = s.k - key0;
+#pragma unroll
+          for (int h = 0; h < HD / 64; ++h)
+            for (int i = valid * 8 + lane; i < kDecTile * 8; i += 32)
+              *reinterpret_cast<uint4*>(tile + C::kTileBytes + h * 2048 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();  // before the stage's next copy
+          __syncwarp();
+        }
         // S = Q K^T: two 8-key column tiles; matrices (keys 0-7 | 8-15) x (k 0-7 | 8-15)
         float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
         {
@@ -330,20 +355,22 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_ke
 #pragma unroll
           for (int k = 0; k < KT; ++k) {
             uint32_t b[4];
-            ldsm4(kt + r * (HD * 2) + (((2 * k + hi) ^ (r & 7)) << 4), b);
+            ldsm4(kt + (k >> 2) * 2048 + r * 128 + (((2 * (k & 3) + hi) ^ (r & 7)) << 4), b);
             mma16816<DT>(s0, qf[k], b[0], b[1]);
             mma16816<DT>(s1, qf[k], b[2], b[3]);
           }
         }
-        const int kc = key0 + (lane & 3) * 2;
-        s0[0] = kc < lim0 ? s0[0] : -INFINITY;
-        s0[1] = kc + 1 < lim0 ? s0[1] : -INFINITY;
-        s1[0] = kc + 8 < lim0 ? s1[0] : -INFINITY;
-        s1[1] = kc + 9 < lim0 ? s1[1] : -INFINITY;
-        s0[2] = kc < lim1 ? s0[2] : -INFINITY;
-        s0[3] = kc + 1 < lim1 ? s0[3] : -INFINITY;
-        s1[2] = kc + 8 < lim1 ? s1[2] : -INFINITY;
-        s1[3] = kc + 9 < lim1 ? s1[3] : -INFINITY;
+        if (key0 + kDecTile > lim_min) {
+          const int kc = key0 + (lane & 3) * 2;
+          s0[0] = kc < lim0 ? s0[0] : -INFINITY;
+          s0[1] = kc + 1 < lim0 ? s0[1] : -INFINITY;
+          s1[0] = kc + 8 < lim0 ? s1[0] : -INFINITY;
+          s1[1] = kc + 9 < lim0 ? s1[1] : -INFINITY;
+          s0[2] = kc < lim1 ? s0[2] : -INFINITY;
+          s0[3] = kc + 1 < lim1 ? s0[3] : -INFINITY;
+          s1[2] = kc + 8 < lim1 ? s1[2] : -INFINITY;
+          s1[3] = kc + 9 < lim1 ? s1[3] : -INFINITY;
+        }
         float t0 = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s1[0], s1[1]));
         float t1 = fmaxf(fmaxf(s0[2], s0[3]), fmaxf(s1[2], s1[3]));
         t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
@@ -390,7 +417,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_ke
 #pragma unroll
           for (int n = 0; n < HD / 16; ++n) {
             uint32_t b[4];
-            ldsm4t(vt + r * (HD * 2) + (((2 * n + hi) ^ (r & 7)) << 4), b);
+            ldsm4t(vt + (n >> 2) * 2048 + r * 128 + (((2 * (n & 3) + hi) ^ (r & 7)) << 4), b);
             mma16816<DT>(o[2 * n], pf, b[0], b[1]);
             mma16816<DT>(o[2 * n + 1], pf, b[2], b[3]);
           }
@@ -398,119 +425,100 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm) paged_decode_ke
       }
       free_stage = stage;
       stage = stage + 1 == C::kStages ? 0 : stage + 1;
+      step(now);
     }
+    // the next item's queries, on their way during the join
+    if (now.left > 0) load_q(now);
 
-    // ---- join the four warps: common maximum, then O summed in warp order
+    // ---- join the four warps, 8 rows at a time: each leaves its maximum, sum
+    // and O; 16 threads per row add them up in warp order
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    const int r0 = lane >> 2, r1 = r0 + 8;
-    if ((lane & 3) == 0) {
-      s_m[warp][r0] = m0;
-      s_m[warp][r1] = m1;
-      s_l[warp][r0] = l0;
-      s_l[warp][r1] = l1;
-    }
-    __syncthreads();
-    float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
+    const int r0 = lane >> 2;
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-      M0 = fmaxf(M0, s_m[w][r0]);
-      M1 = fmaxf(M1, s_m[w][r1]);
-    }
+    for (int half = 0; half < 2; ++half) {
+      if (half * 8 >= rows) break;
+      __syncthreads();  // the buffer's last readers are done
+      // column groups of 8 are permuted by row, which spreads the banks
+      float* so = s_o + (warp * 8 + r0) * HD;
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-      L0 += s_m[w][r0] == -INFINITY ? 0.f : s_l[w][r0] * ex2_f32(s_m[w][r0] - M0);
-      L1 += s_m[w][r1] == -INFINITY ? 0.f : s_l[w][r1] * ex2_f32(s_m[w][r1] - M1);
-    }
-    const float f0 = m0 == -INFINITY ? 0.f : ex2_f32(m0 - M0);
-    const float f1 = m1 == -INFINITY ? 0.f : ex2_f32(m1 - M1);
-#pragma unroll
-    for (int i = 0; i < HD / 8; ++i) {
-      o[i][0] *= f0;
-      o[i][1] *= f0;
-      o[i][2] *= f1;
-      o[i][3] *= f1;
-    }
-    // warps 2, 3 -> 0, 1, then 1 -> 0
-    const int slot = warp & 1;
-    float* so = s_o + slot * (kDecRows * HD);
-    auto put = [&](float* dst) {
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) {
-        *reinterpret_cast<float2*>(dst + (i * 32 + lane) * 4) = make_float2(o[i][0], o[i][1]);
-        *reinterpret_cast<float2*>(dst + (i * 32 + lane) * 4 + 2) = make_float2(o[i][2], o[i][3]);
+      for (int i = 0; i < HD / 8; ++i)
+        *reinterpret_cast<float2*>(so + ((i ^ (r0 & 3)) * 8) + (lane & 3) * 2) =
+            make_float2(o[i][2 * half], o[i][2 * half + 1]);
+      if ((lane & 3) == 0) {
+        s_m[warp][r0] = half ? m1 : m0;
+        s_l[warp][r0] = half ? l1 : l0;
       }
-    };
-    auto add = [&](const float* src) {
+      __syncthreads();
+      const int row = threadIdx.x >> 4;  // 0..7
+      const int r = half * 8 + row;
+      if (r < rows) {
+        float M = -INFINITY, L = 0.f, f[kDecWarps];
 #pragma unroll
-      for (int i = 0; i < HD / 8; ++i) {
-        const float4 x = *reinterpret_cast<const float4*>(src + (i * 32 + lane) * 4);
-        o[i][0] += x.x;
-        o[i][1] += x.y;
-        o[i][2] += x.z;
-        o[i][3] += x.w;
-      }
-    };
-    if (warp >= 2) put(so);
-    __syncthreads();
-    if (warp < 2) add(so);
-    if (warp == 1) put(so);
-    __syncthreads();
-    if (warp == 0) {
-      add(s_o + kDecRows * HD);
-      const float i0 = L0 > 0.f ? 1.f / L0 : 0.f, i1 = L1 > 0.f ? 1.f / L1 : 0.f;
-      const float g0 = L0 > 0.f ? M0 + __log2f(L0) : -INFINITY, g1 = L1 > 0.f ? M1 + __log2f(L1) : -INFINITY;
+        for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][row]);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = half ? r1 : r0;
-        if (r >= rows) continue;
-        const float inv = half ? i1 : i0, lg = half ? g1 : g0;
+        for (int w = 0; w < kDecWarps; ++w) {
+          f[w] = s_m[w][row] == -INFINITY ? 0.f : ex2_f32(s_m[w][row] - M);
+          L += s_l[w][row] * f[w];
+        }
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+        const float lg = L > 0.f ? M + __log2f(L) : -INFINITY;
         const int tok = s.q0 + r / p.group, head = kvh * p.group + r % p.group;
-        if (whole) {
-          const long long base = static_cast<long long>(tok) * a.o_ts + static_cast<long long>(head) * a.o_hs + (lane & 3) * 2;
-          if (a.out_f32) {
+        const int col = threadIdx.x & 15;
+        const long long place = 2ll * blockIdx.x + (earlier ? 1 : 0);
 #pragma unroll
-            for (int i = 0; i < HD / 8; ++i)
-              *reinterpret_cast<float2*>(static_cast<float*>(a.out) + base + i * 8) =
-                  make_float2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
-          } else {
+        for (int g = 0; g < HD / 64; ++g) {  // 4 columns each
+          const int cc = (g * 16 + col) * 4;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < HD / 8; ++i)
-              *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + base + i * 8) =
-                  pack2<DT>(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
+          for (int w = 0; w < kDecWarps; ++w) {
+            const float4 y = *reinterpret_cast<const float4*>(s_o + (w * 8 + row) * HD + (cc ^ ((row & 3) * 8)));
+            x.x = fmaf(y.x, f[w], x.x);
+            x.y = fmaf(y.y, f[w], x.y);
+            x.z = fmaf(y.z, f[w], x.z);
+            x.w = fmaf(y.w, f[w], x.w);
           }
-          if (a.lse != nullptr && (lane & 3) == 0)
+          x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+          if (!whole) {
+            *reinterpret_cast<float4*>(p.o_part + (place * kDecRows + r) * HD + cc) = x;
+          } else if (a.out_f32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + static_cast<long long>(tok) * a.o_ts +
+                                       static_cast<long long>(head) * a.o_hs + cc) = x;
+          } else {
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + static_cast<long long>(tok) * a.o_ts +
+                                      static_cast<long long>(head) * a.o_hs + cc) =
+                make_uint2(pack2<DT>(x.x, x.y), pack2<DT>(x.z, x.w));
+          }
+        }
+        if (col == 0) {
+          if (!whole) {
+            p.l_part[place * kDecRows + r] = lg;
+          } else if (a.lse != nullptr) {
             a.lse[static_cast<long long>(head) * a.tokens + tok] = lg * 0.69314718055994531f;
-        } else {
-          const long long part = 2ll * blockIdx.x + (first_segment ? 0 : 1);
-          float* dst = p.o_part + (part * kDecRows + r) * HD + (lane & 3) * 2;
-#pragma unroll
-          for (int i = 0; i < HD / 8; ++i)
-            *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
-          if ((lane & 3) == 0) p.l_part[part * kDecRows + r] = lg;
+          }
         }
       }
     }
-    // on to the next item (or to the end)
-    first_segment = false;
-    now.c = c_end - 1;
-    advance(now, step < steps);
   }
-  cp_wait<0>();
 }
 
 // Joins the partial results of every item that more than one block worked on,
 // and writes the rows of sequences without keys (out 0, log-sum-exp -inf).
-// One block per (sequence, key head) and row; its warps take every fourth
-// partial result, so that long joins are not a chain of memory latencies, and
-// add up in warp order.
+// One block per (sequence, key head) and row: the weights of all partial
+// results first, then each warp adds up every eighth result, eight of them
+// requested at a time, and the warps' sums are added in warp order. What
+// bounds it is the chain of latencies (lengths, weights, results), so a long
+// join is spread over the warps.
+constexpr int kJoinWarps = 8;
+
 template <int HD, int DT>
-__global__ void __launch_bounds__(kDecWarps * 32) paged_combine_kernel(const DecodeK p, int blocks) {
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_combine_kernel(const __grid_constant__ DecodeK p, int blocks) {
   constexpr int E = HD / 32;
-  __shared__ float s_o[kDecWarps][HD];
-  __shared__ float s_l[kDecWarps];
+  extern __shared__ float s_w[];  // [blocks] weights
+  __shared__ float s_o[kJoinWarps][HD];
+  __shared__ float s_l[kJoinWarps], s_max[kJoinWarps];
   const SeqArgs& a = p.a;
   pdl_wait();
   pdl_trigger();
@@ -521,63 +529,77 @@ __global__ void __launch_bounds__(kDecWarps * 32) paged_combine_kernel(const Dec
   if (s.bad && kvh == 0 && r == 0 && threadIdx.x == 0) record_error(p.status, kDevBadIndex);
   if (r >= s.q * p.group) return;
   const int nu = units_of(s);
-  int c0 = 0, c1 = -1;
-  long long ua = 0;
-  Runs runs(0, 1);
+  int c0 = 0, n = 0;  // the item's blocks
+  bool late = false;
   if (nu > 0) {
-    long long all = 0, mine = 0;  // units of all sequences, and of those before this one
+    int all = 0, mine = 0;  // places of all sequences, and of those before this one
 #pragma unroll 4
     for (int b = lane; b < a.batch; b += 32) {
-      const int n = units_of(decode_lens(a, p.group, p.page_shift, b));
-      all += n;
-      mine += b < seq ? n : 0;
+      const int x = places_of(decode_lens(a, p.group, p.page_shift, b));
+      all += x;
+      mine += b < seq ? x : 0;
     }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-      all += __shfl_xor_sync(0xffffffffu, all, d);
-      mine += __shfl_xor_sync(0xffffffffu, mine, d);
-    }
-    runs = Runs(all * a.kv_heads, blocks);
-    ua = mine * a.kv_heads + static_cast<long long>(kvh) * nu;
+    const Runs runs(__reduce_add_sync(0xffffffffu, all) * a.kv_heads, blocks);
+    const int ua = __reduce_add_sync(0xffffffffu, mine) * a.kv_heads + kvh * (nu + kSegment);
     c0 = runs.block_of(ua);
-    c1 = runs.block_of(ua + nu - 1);
-    if (c0 == c1) return;  // one block saw all of it and wrote the result
+    n = runs.block_of(ua + nu - 1) - c0 + 1;
+    if (n == 1) return;  // one block saw all of it and wrote the result
+    // block c's partial result is in its first place, unless its run began
+    // before the item (only c0's can have)
+    late = runs.start(c0) < ua;
   }
-  // partial result of block c: its first segment's place, unless the block
-  // began with an earlier item (only c0 can have)
-  const bool late = runs.start(c0) < ua;
-  auto part = [&](int c) { return 2ll * c + (late && c == c0 ? 1 : 0); };
+  auto part = [&](int i) { return 2ll * (c0 + i) + (late && i == 0 ? 1 : 0); };
   float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.l_part[part(c) * kDecRows + r]);
+  for (int i = threadIdx.x; i < n; i += kJoinWarps * 32) {
+    s_w[i] = p.l_part[part(i) * kDecRows + r];
+    m = fmaxf(m, s_w[i]);
+  }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if (lane == 0) s_max[warp] = m;
+  __syncthreads();
+  m = s_max[0];
+#pragma unroll
+  for (int w = 1; w < kJoinWarps; ++w) m = fmaxf(m, s_max[w]);
   float l = 0.f, acc[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += kDecWarps) {
-    const float lg = p.l_part[part(c) * kDecRows + r];
-    const float w = lg == -INFINITY ? 0.f : ex2_f32(lg - m);
-    const float* src = p.o_part + (part(c) * kDecRows + r) * HD + lane * E;
+#pragma unroll 8
+  for (int i = warp; i < n; i += kJoinWarps) {
+    const float w = s_w[i] == -INFINITY ? 0.f : ex2_f32(s_w[i] - m);
+    const float* src = p.o_part + (part(i) * kDecRows + r) * HD + lane * E;
     l += w;
-#pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = fmaf(w, src[i], acc[i]);
+    if constexpr (E == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(src);
+      acc[0] = fmaf(w, x.x, acc[0]);
+      acc[1] = fmaf(w, x.y, acc[1]);
+      acc[2] = fmaf(w, x.z, acc[2]);
+      acc[3] = fmaf(w, x.w, acc[3]);
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(src);
+      acc[0] = fmaf(w, x.x, acc[0]);
+      acc[1] = fmaf(w, x.y, acc[1]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < E; ++i) s_o[warp][lane * E + i] = acc[i];
   if (lane == 0) s_l[warp] = l;
   __syncthreads();
-  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (threadIdx.x >= HD) return;
+  float x = 0.f;
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    l += s_l[w];
+    x += s_o[w][threadIdx.x];
+  }
+  x = l > 0.f ? x / l : 0.f;
   const int tok = s.q0 + r / p.group, head = kvh * p.group + r % p.group;
-  const long long base = static_cast<long long>(tok) * a.o_ts + static_cast<long long>(head) * a.o_hs;
-  for (int i = threadIdx.x; i < HD; i += kDecWarps * 32) {
-    const float x = ((s_o[0][i] + s_o[1][i]) + (s_o[2][i] + s_o[3][i])) * inv;
-    if (a.out_f32) {
-      static_cast<float*>(a.out)[base + i] = x;
-    } else {
-      static_cast<uint16_t*>(a.out)[base + i] = static_cast<uint16_t>(pack2<DT>(x, 0.f) & 0xffffu);
-    }
+  const long long at = static_cast<long long>(tok) * a.o_ts + static_cast<long long>(head) * a.o_hs + threadIdx.x;
+  if (a.out_f32) {
+    static_cast<float*>(a.out)[at] = x;
+  } else {
+    static_cast<uint16_t*>(a.out)[at] = static_cast<uint16_t>(pack2<DT>(x, 0.f) & 0xffffu);
   }
   if (a.lse != nullptr && threadIdx.x == 0)
     a.lse[static_cast<long long>(head) * a.tokens + tok] =
@@ -586,13 +608,13 @@ __global__ void __launch_bounds__(kDecWarps * 32) paged_combine_kernel(const Dec
 
 // Blocks of a call: every SM's share, but no more than there can be units.
 int decode_blocks(const SeqArgs& a) {
-  const long long units = (a.max_k + kDecUnit - 1) / kDecUnit * a.batch * a.kv_heads;
+  const long long units = ((a.max_k + kDecUnit - 1) / kDecUnit) * a.batch * a.kv_heads;
   const long long most = static_cast<long long>(kDecCtasPerSm) * device_sm_count();
   return static_cast<int>(units < 1 ? 1 : units < most ? units : most);
 }
 
 template <int HD, int DT>
-int launch_decode(const DecodeK& k, int blocks, cudaStream_t stream) {
+int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeK& k, int blocks, cudaStream_t stream) {
   using C = DecCfg<HD>;
   auto kern = paged_decode_kernel<HD, DT>;
   static bool attr_done[64] = {};
@@ -603,11 +625,11 @@ int launch_decode(const DecodeK& k, int blocks, cudaStream_t stream) {
     if (e != cudaSuccess) return set_error(TF_ERR_LAUNCH, "cudaFuncSetAttribute(paged decode): %s", cudaGetErrorString(e));
     attr_done[dev & 63] = true;
   }
-  cudaError_t e = launch_k(kern, dim3(blocks), dim3(kDecWarps * 32), C::kBytes, stream, k);
+  cudaError_t e = launch_k(kern, dim3(blocks), dim3(kDecWarps * 32), C::kBytes, stream, tk, tv, k);
   if (e == cudaSuccess)
     e = launch_k(paged_combine_kernel<HD, DT>,
                  dim3(static_cast<unsigned>(k.a.batch * k.a.kv_heads), static_cast<unsigned>(k.a.max_q * k.group)),
-                 dim3(kDecWarps * 32), 0, stream, k, blocks);
+                 dim3(kJoinWarps * 32), blocks * sizeof(float), stream, k, blocks);
   if (e != cudaSuccess) return set_error(TF_ERR_LAUNCH, "paged decode launch: %s", cudaGetErrorString(e));
   return TF_OK;
 }
@@ -621,6 +643,8 @@ long long paged_decode_workspace(const SeqArgs& a) {
 }
 
 int paged_decode(const SeqArgs& a, cudaStream_t stream) {
+  if ((a.max_pages * a.page_size / kDecUnit + 1 + kSegment) * a.batch * a.kv_heads >= (1ll << 31))
+    return set_error(TF_ERR_SHAPE, "paged attention: a table of %lld x %lld pages is out of range", a.batch, a.max_pages);
   DecodeK k = {};
   k.a = a;
   k.group = a.heads / a.kv_heads;
@@ -631,9 +655,18 @@ int paged_decode(const SeqArgs& a, cudaStream_t stream) {
   k.l_part = k.o_part + static_cast<long long>(blocks) * 2 * kDecRows * a.head_dim;
   k.status = device_status_ptr();
   if (k.status == nullptr) return last_error_code();
+  CUtensorMap tk, tv;
+  int rc = make_tmap_4d_f16(&tk, a.k, {a.head_dim, a.kv_heads, a.page_size, a.num_pages}, {a.k_hs, a.k_ts, a.k_ps},
+                            {64, 1, kDecTile, 1});
+  if (rc) return rc;
+  rc = make_tmap_4d_f16(&tv, a.v, {a.head_dim, a.kv_heads, a.page_size, a.num_pages}, {a.v_hs, a.v_ts, a.v_ps},
+                        {64, 1, kDecTile, 1});
+  if (rc) return rc;
   if (a.bf16)
-    return a.head_dim == 64 ? launch_decode<64, kDtBF16>(k, blocks, stream) : launch_decode<128, kDtBF16>(k, blocks, stream);
-  return a.head_dim == 64 ? launch_decode<64, kDtF16>(k, blocks, stream) : launch_decode<128, kDtF16>(k, blocks, stream);
+    return a.head_dim == 64 ? launch_decode<64, kDtBF16>(tk, tv, k, blocks, stream)
+                            : launch_decode<128, kDtBF16>(tk, tv, k, blocks, stream);
+  return a.head_dim == 64 ? launch_decode<64, kDtF16>(tk, tv, k, blocks, stream)
+                          : launch_decode<128, kDtF16>(tk, tv, k, blocks, stream);
 }
 
 }  // namespace tfb
