@@ -131,7 +131,9 @@ def check(fn: str, rc: int) -> None:
 
 def call(fn: str, *args) -> None:
     """Call an ABI function and raise TfError on a non-zero status."""
-    check(fn, getattr(load(), fn)(*args))
+    rc = getattr(_lib or load(), fn)(*args)
+    if rc != TF_OK:
+        check(fn, rc)
 
 
 def call_value(fn: str, *args) -> int:

@@ -8,6 +8,7 @@ tensor on the CPU, a wrong dtype or a missing library raises.
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -502,7 +503,7 @@ def _rotary_operands(name, q, k, positions, freqs):
 
 def _rotary_out(name, what, x, out):
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return x.new_empty(x.shape)
     _need_heads(name, what, out, x.dtype)
     if out.shape != x.shape:
         raise ValueError(f"{name}: {what} must have its input's shape")
@@ -588,14 +589,14 @@ def _seq_operands(name, q, kv_heads, cu_q, max_q, scale, out, out_dtype, lse, wa
     if out_dtype not in (q.dtype, torch.float32):
         raise ValueError(f"{name}: out_dtype must be q's type or fp32")
     if out is None:
-        out = torch.empty(t, h, hd, dtype=out_dtype, device=q.device)
+        out = q.new_empty(q.shape, dtype=out_dtype)
     else:
         _need_heads(name, "out", out, out_dtype)
         if out.shape != q.shape:
             raise ValueError(f"{name}: out must have q's shape")
     if lse is None:
         if want_lse:
-            lse = torch.empty(h, t, dtype=torch.float32, device=q.device)
+            lse = q.new_empty((h, t), dtype=torch.float32)
     elif lse.dtype != torch.float32 or lse.shape != (h, t) or not lse.is_contiguous():
         raise ValueError(f"{name}: lse must be contiguous fp32 [heads, tokens]")
     flags = (_abi.TF_ATTN_OUT_F32 if out_dtype == torch.float32 else 0) | (
@@ -603,16 +604,17 @@ def _seq_operands(name, q, kv_heads, cu_q, max_q, scale, out, out_dtype, lse, wa
     return out, lse, flags
 
 
-def _seq_workspace(name, fn, dev, workspace, *sizes):
-    if dev == torch._C._cuda_getDevice():
-        need = _abi.call_value(fn, *sizes)
-    else:
-        with torch.cuda.device(dev):
-            need = _abi.call_value(fn, *sizes)
+@functools.lru_cache(maxsize=4096)
+def _seq_workspace_bytes(dev: int, fn: str, *sizes: int) -> int:
+    """A size depends on the call's sizes and the device alone."""
+    with torch.cuda.device(dev):
+        return _abi.call_value(fn, *sizes)
+
+
+def _seq_workspace(name, fn, dev, like, workspace, *sizes):
+    need = _seq_workspace_bytes(dev, fn, *sizes)
     if workspace is None:
-        if need == 0:
-            return None, 0
-        return torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev)), need
+        return (like.new_empty(need, dtype=torch.uint8), need) if need else (None, 0)
     if not workspace.is_contiguous() or workspace.get_device() != dev:
         raise ValueError(f"{name}: workspace must be contiguous, on the operands' device")
     size = workspace.numel() * workspace.element_size()
@@ -653,7 +655,7 @@ def flash_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu
         raise ValueError(f"{name}: max_k must not be negative")
     dev = _device_of(name, q, k, v, cu_q, cu_k, out, lse)
     (t, h, hd), (tk, g, _), b = q.shape, k.shape, cu_q.shape[0] - 1
-    ws, ws_bytes = _seq_workspace(name, "tf_flash_packed_workspace", dev, workspace, t, b, h, g, hd, max_q, max_k)
+    ws, ws_bytes = _seq_workspace(name, "tf_flash_packed_workspace", dev, q, workspace, t, b, h, g, hd, max_q, max_k)
     _launch(dev, "tf_flash_packed", q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
             *v.stride()[:2], cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), *out.stride()[:2], _ptr(lse), t, tk, b, h,
             g, hd, max_q, max_k, scale, flags | (_abi.TF_ATTN_CAUSAL if causal else 0), _ptr(ws), ws_bytes)
@@ -696,7 +698,7 @@ def flash_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         raise ValueError(f"{name}: max_kv must not be negative")
     dev = _device_of(name, q, k_cache, v_cache, page_table, cu_q, kv_lens, out, lse)
     t, h, hd = q.shape
-    ws, ws_bytes = _seq_workspace(name, "tf_flash_paged_workspace", dev, workspace, t, b, h, g, hd, max_q, max_kv)
+    ws, ws_bytes = _seq_workspace(name, "tf_flash_paged_workspace", dev, q, workspace, t, b, h, g, hd, max_q, max_kv)
     _launch(dev, "tf_flash_paged", q.data_ptr(), *q.stride()[:2], k_cache.data_ptr(), v_cache.data_ptr(),
             *k_cache.stride()[:3], pages, page, page_table.data_ptr(), page_table.stride()[0], max_pages,
             cu_q.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), *out.stride()[:2], _ptr(lse), t, b, h, g, hd, max_q,
