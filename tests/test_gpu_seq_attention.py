@@ -114,6 +114,34 @@ def test_packed(q_lens, k_lens, h, g, hd, causal, dtype):
     check_packed(q, k, v, cu_q, cu_k, hd ** -0.5, causal, out32, None)
 
 
+def spread(n, lo, hi, seed):
+    gen = torch.Generator().manual_seed(seed)
+    return torch.randint(lo, hi, (n,), generator=gen).tolist()
+
+
+LISTED = [  # more items than SMs: listed tiles, the last with long keys cut into ranges
+    (spread(60, 1, 700, 1), None, 8, 4, 64, True), (spread(70, 0, 300, 2), spread(70, 0, 500, 3), 12, 4, 128, False),
+    ([40, 3000, 500, 2900], [3500, 3000, 2600, 4000], 16, 4, 64, True),
+    ([900, 1, 1, 1, 700], [2500, 5000, 4000, 17, 3000], 24, 8, 128, True),
+    ([1000, 0, 600], [4100, 3, 6000], 10, 5, 64, False), (spread(1100, 0, 71, 4), None, 8, 1, 64, True),
+    (spread(1300, 1, 4, 5), spread(1300, 0, 300, 6), 4, 4, 64, True),
+    ([2500, 2400], None, 16, 16, 64, True),  # asks for more ranges than there are places for
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_lens,k_lens,h,g,hd,causal", LISTED)
+def test_packed_listed(q_lens, k_lens, h, g, hd, causal):
+    k_lens = q_lens if k_lens is None else k_lens
+    q, k, v, cu_q, cu_k = packed_case(q_lens, k_lens, h, g, hd, BF16, peak=2.0)
+    args = (q, k, v, cu_q, cu_k, max(q_lens), hd ** -0.5)
+    out, lse = K.flash_attention_packed(*args, causal=causal, want_lse=True, max_k=max(k_lens))
+    check_packed(q, k, v, cu_q, cu_k, hd ** -0.5, causal, out, lse)
+    for _ in range(10):  # the draw of items depends on timing, results do not
+        again, lse2 = K.flash_attention_packed(*args, causal=causal, want_lse=True, max_k=max(k_lens))
+        assert torch.equal(again, out) and torch.equal(lse2, lse)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("causal", [False, True])
@@ -215,7 +243,7 @@ PAGED = [  # q_lens, kv_lens, heads, kv_heads, hd, page
     ([1, 1], [20000, 3], 3, 3, 64, 256), ([1], [9000], 16, 1, 128, 16), ([16], [500], 3, 3, 64, 16),
     ([40, 1, 300], [40, 700, 1000], 8, 2, 64, 16), ([129, 5], [640, 5], 4, 4, 128, 32),
     ([17, 1, 1, 64], [17, 129, 5000, 200], 5, 1, 64, 64), ([300, 2], [300, 100], 14, 2, 128, 128),
-    ([33, 20], [32, 4000], 8, 8, 128, 512), ([5], [7000], 32, 4, 64, 16), ([200, 0, 1], [0, 0, 333], 6, 2, 64, 16),
+    ([33, 20], [32, 4000], 8, 8, 128, 512), ([1] * 30 + [300, 170], [1 + 61 * i for i in range(30)] + [2000, 4000], 32, 8, 64, 32), ([5], [7000], 32, 4, 64, 16), ([200, 0, 1], [0, 0, 333], 6, 2, 64, 16),
 ]
 
 

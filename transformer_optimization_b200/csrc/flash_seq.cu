@@ -14,10 +14,20 @@
 //   over [token][key head][group head][64 columns] fills 128 / G tokens times
 //   G heads per tile in one copy. G heads of one token see the same keys, so
 //   the causal limit is per token and a tile spans fewer positions.
-// * Tiles are cut per sequence. A CTA finds its (sequence, tile) by a warp
-//   scan over the offsets (32 sequences per step), so the call needs no plan,
-//   no host copy of the lengths and nothing kept from call to call; the grid
-//   is the bound tokens / tile + batch, and CTAs past the last tile leave.
+// * Tiles are cut per sequence, and a CTA works on one after another: an item
+//   is (two tiles of a sequence, key head, key range). The warps' rings and
+//   barriers run on across items, so the next item's Q, K and V arrive and its
+//   first scores are formed while the last one's softmax and stores still run
+//   (a CTA per item spent 5.5 us, hd 64, to 7.5 us, hd 128, on start and end,
+//   as long as four key blocks take).
+// * More items than SMs: seq_plan_kernel lists the tiles by falling cost, and
+//   CTAs draw items from the list by a counter, so that a long item never
+//   starts last; where keys are long, items late in the list are cut into key
+//   ranges (guided by the work that is left), so that the last ones end
+//   together. Fewer items than SMs: CTA c takes item c, found by a warp scan
+//   over the offsets, and every tile is cut into the same number of ranges.
+//   Either way the call needs no host copy of the lengths and keeps nothing,
+//   and the cuts depend on the lengths alone, so results repeat bit for bit.
 // * Key blocks start at the sequence's first key, and a copy may run into the
 //   next sequence or past a page's end. Such scores are masked as usual; such
 //   V rows are zeroed in shared memory before the product (0 * NaN would
@@ -26,9 +36,8 @@
 // * Paged: a key block is 128 / page_size copies, one per page (one copy of a
 //   part of a larger page), issued by as many lanes; page indices are read one
 //   block ahead. An index outside the cache reads zeros and is reported.
-// * Few tiles and long keys: the key blocks of each tile are cut into
-//   `splits` ranges, whose normalised fp32 results and log-sum-exps
-//   seq_combine_kernel joins in range order.
+// * A range leaves its normalised fp32 result and log-sum-exp in a slot of the
+//   workspace; seq_combine_kernel joins a tile's ranges in range order.
 #include "attn_common.cuh"
 #include "common.cuh"
 #include "launch.h"
@@ -36,10 +45,18 @@
 namespace tfb {
 namespace {
 
-struct SeqK {
+// Where results go.
+struct SeqOut {
   void* out;
   long long o_ts, o_hs;
   float* lse;
+  float* o_part;    // [slot][key head][256 rows][HD]
+  float* lse_part;  // [slot][key head][256 rows], natural log
+  int tokens, out_f32;
+};
+
+struct SeqK {
+  SeqOut o;
   const int* cu_q;
   const int* cu_k;
   const int* kv_lens;
@@ -49,26 +66,40 @@ struct SeqK {
   long long page_cap;                   // keys a page table row can hold
   int batch, heads, group, tokens, k_tokens, max_q;
   int tok_tile;  // tokens per 128-row tile
-  int splits;
-  float* o_part;    // [splits][tokens][heads][HD]
-  float* lse_part;  // [splits][tokens][heads], natural log
+  int splits;    // without a plan: key ranges per tile
   float scale_log2;
-  int causal, out_f32;
+  int causal;
+  int kv_heads, max_tiles;
+  int max_slots;  // with a plan: slots for key ranges, 0 when tiles are not cut
+  // The plan, null when there are no more items than SMs: ints 0 entries, 1
+  // next item, 2 cut tiles; from kPlanHead on the first entry of each cut tile
+  // (max_slots / 2), the tiles in order (max_tiles) and, if tiles are cut, the
+  // entries (max_tiles + max_slots).
+  int* plan;
   int* status;
 };
+
+// Register split (see attn_common.cuh): the item loop needs 56 registers in
+// the producer and MMA warps, and the softmax fits 224.
+constexpr int kSeqRegsLow = 56;
+constexpr int kSeqRegsHigh = 224;
+static_assert(128 * kSeqRegsLow + 256 * kSeqRegsHigh <= kAttnThreads * kRegsLaunch, "register split exceeds the pool");
+
+constexpr int kPlanHead = 8;  // ints before the plan's tiles
 
 template <int HD>
 struct SeqCfg {
   static constexpr int kNS = HD == 64 ? 3 : 2;
+  static constexpr int kNQ = HD == 64 ? 2 : 1;      // items whose queries fit
   static constexpr int kStages = HD == 64 ? 4 : 2;  // of K and of V
   static constexpr int kTileBytes = 128 * HD * 2;
   static constexpr int kQOff = 0;
-  static constexpr int kKOff = kQOff + kAttnTiles * kTileBytes;
+  static constexpr int kKOff = kQOff + kNQ * kAttnTiles * kTileBytes;
   static constexpr int kVOff = kKOff + kStages * kTileBytes;
   static constexpr int kBarOff = kVOff + kStages * kTileBytes;
-  // q_full, v_tail, k_full/empty, v_full/empty, s_full[NS], p_full[2 x 2],
-  // turn[2], drain[2], pv_done[NS]
-  static constexpr int kNumBars = 2 + 4 * kStages + kNS + 4 + 2 + 2 + kNS;
+  // item_full/empty[2], s_done[2], q_full/empty[NQ], v_tail, k_full/empty, v_full/empty,
+  // s_full[NS], p_full[NS], turn[2], drain[2], pv_done[NS]
+  static constexpr int kNumBars = 6 + 2 * kNQ + 1 + 4 * kStages + 3 * kNS + 2 + 2;
   static constexpr int kBytes = kBarOff + kNumBars * 8 + 16;
   static constexpr int kAlloc = kBytes + 1024;
   static constexpr uint32_t kTmS = 0;
@@ -77,19 +108,32 @@ struct SeqCfg {
 };
 
 struct SeqWork {
-  int seq, tile;    // seq < 0: no work
-  int q0, q_len;    // first query token, queries
-  int k0, k_len;    // packed: first key token; keys
+  int seq, tile;  // seq < 0: no work
+  int q0, q_len;  // first query token, queries
+  int k0, k_len;  // packed: first key token; keys
+  int jb, je;     // key blocks
+  int slot;       // where the range's partial result goes; -1: the range is all
+  int kvh;        // key head
+  int ranges;     // of the tile
+  int cost;       // (plan)
 };
+static_assert(sizeof(SeqWork) == 48, "a plan entry");
+
+__device__ __forceinline__ int* plan_joins(const SeqK& p) { return p.plan + kPlanHead; }
+__device__ __forceinline__ SeqWork* plan_tiles(const SeqK& p) {
+  return reinterpret_cast<SeqWork*>(p.plan + kPlanHead + p.max_slots / 2);
+}
+__device__ __forceinline__ SeqWork* plan_entries(const SeqK& p) {
+  return plan_tiles(p) + (p.max_slots > 0 ? p.max_tiles : 0);
+}
 
 // Queries and keys of sequence b, bounded by what the call's arrays hold. A
 // bound that bites is an error of the caller's: it is reported, and nothing
 // outside the arrays is read or written.
 template <bool PAGED>
 __device__ __forceinline__ SeqWork seq_lens(const SeqK& p, int b, bool& bad) {
-  SeqWork w;
+  SeqWork w = {};
   w.seq = b;
-  w.tile = 0;
   const int c0 = p.cu_q[b], c1 = p.cu_q[b + 1];
   w.q0 = min(max(c0, 0), p.tokens);
   w.q_len = min(min(max(c1, w.q0), p.tokens) - w.q0, p.max_q);
@@ -133,7 +177,7 @@ __device__ __forceinline__ SeqWork find_tile(const SeqK& p, int at) {
     const unsigned hit = __ballot_sync(0xffffffffu, run + inc > at);
     if (hit != 0) {
       const int l = __ffs(hit) - 1;
-      SeqWork r;
+      SeqWork r = {};
       r.seq = base + l;
       r.tile = at - run - __shfl_sync(0xffffffffu, inc - n, l);
       r.q0 = __shfl_sync(0xffffffffu, w.q0, l);
@@ -149,6 +193,259 @@ __device__ __forceinline__ SeqWork find_tile(const SeqK& p, int at) {
   return none;
 }
 
+// The item's key blocks: n0 and n1 of its two tiles, from block jb on.
+struct SeqBlocks {
+  int tok0;   // first token, within the sequence
+  int shift;  // query i stands at key i + shift
+  int n0, n1;
+  __device__ __forceinline__ int most() const { return max(n0, n1); }
+  __device__ __forceinline__ int both() const { return min(n0, n1); }
+};
+__device__ __forceinline__ int tile_blocks(const SeqK& p, const SeqWork& w, int t0) {
+  int k_end = t0 < w.q_len ? w.k_len : 0;
+  if (p.causal && k_end > 0) k_end = min(k_end, min(t0 + p.tok_tile, w.q_len) + w.k_len - w.q_len);
+  return k_end <= 0 ? 0 : (k_end + kAttnBN - 1) / kAttnBN;
+}
+__device__ __forceinline__ SeqBlocks seq_blocks(const SeqK& p, const SeqWork& w) {
+  SeqBlocks g;
+  g.tok0 = w.tile * 2 * p.tok_tile;
+  g.shift = w.k_len - w.q_len;
+  g.n0 = max(min(tile_blocks(p, w, g.tok0), w.je) - w.jb, 0);
+  g.n1 = max(min(tile_blocks(p, w, g.tok0 + p.tok_tile), w.je) - w.jb, 0);
+  return g;
+}
+
+// ---------------------------------------------------------------------------
+// plan
+// ---------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 1024;
+constexpr int kClasses = 64;
+// Costs in fifths of a key block of two tiles: such a block, one of a tile
+// alone, an item's start and end. Measured: 1.6 us, about 1 us, about 3 us.
+constexpr int kCostBlock = 5, kCostHalf = 3, kCostItem = 10;
+constexpr int kMinRange = 6;  // key blocks; a shorter range costs more than it evens out
+
+// Inclusive sum over the block's threads; `total` is the block's.
+template <typename T>
+__device__ __forceinline__ T block_scan(T x, T* s_warp, T& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const T up = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += up;
+  }
+  if (lane == 31) s_warp[warp] = x;
+  __syncthreads();
+  T w = s_warp[lane];
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const T up = __shfl_up_sync(0xffffffffu, w, d);
+    if (lane >= d) w += up;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const T before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  __syncthreads();
+  return x + (warp > 0 ? before : T(0));
+}
+
+// Lists the call's tiles by falling cost: a stable counting sort over kClasses
+// classes of the number of key blocks. Then, if tiles may be cut, walks the
+// list: a tile with the work R left from it on (over all key heads) is cut
+// into ranges of about R / (2 * CTAs), so the ranges shrink with what is left
+// and the last ones end together. One block.
+template <bool PAGED>
+__global__ void __launch_bounds__(kPlanThreads) seq_plan_kernel(const __grid_constant__ SeqK p, int ctas) {
+  __shared__ int s_q0[kPlanThreads], s_q[kPlanThreads], s_k0[kPlanThreads], s_k[kPlanThreads];
+  __shared__ int s_end[kPlanThreads];              // tiles of the chunk's sequences up to each
+  __shared__ int s_count[kPlanThreads / 32][kClasses];  // of each warp's tiles, then tiles before them
+  __shared__ int s_base[kClasses];                 // place of the class's next tile
+  __shared__ int s_warp[32];
+  __shared__ long long s_warp64[32];
+  __shared__ int s_most;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int span = 2 * p.tok_tile;
+  if (tid < kClasses) s_base[tid] = 0;
+  if (tid == 0) s_most = 1;
+  pdl_wait();
+  pdl_trigger();
+  __syncthreads();
+  int most = 1;
+  for (int b = tid; b < p.batch; b += kPlanThreads) {
+    bool bad;
+    const SeqWork w = seq_lens<PAGED>(p, b, bad);
+    if (bad) record_error(p.status, kDevBadIndex);
+    if (w.q_len > 0) most = max(most, tile_blocks(p, w, (w.q_len - 1) / p.tok_tile * p.tok_tile));
+    if (b < kPlanThreads) {
+      s_q0[tid] = w.q0;
+      s_q[tid] = w.q_len;
+      s_k0[tid] = w.k0;
+      s_k[tid] = w.k_len;
+    }
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) atomicMax(&s_most, most);
+  __syncthreads();
+  most = s_most;
+
+  int total = 0;           // tiles
+  long long work = 0;      // this thread's tiles' cost
+  // pass 0 counts the classes, pass 1 places the tiles
+  for (int pass = 0; pass < 2; ++pass) {
+    total = 0;
+    for (int base = 0; base < p.batch; base += kPlanThreads) {
+      if (p.batch > kPlanThreads) {
+        SeqWork w = {};
+        bool bad;
+        if (base + tid < p.batch) w = seq_lens<PAGED>(p, base + tid, bad);
+        s_q0[tid] = w.q0;
+        s_q[tid] = w.q_len;
+        s_k0[tid] = w.k0;
+        s_k[tid] = w.k_len;
+      }
+      int chunk;
+      if (pass == 0 || p.batch > kPlanThreads) {
+        const int n = base + tid < p.batch ? (s_q[tid] + span - 1) / span : 0;
+        s_end[tid] = block_scan(n, s_warp, chunk);
+        __syncthreads();
+      }
+      chunk = s_end[kPlanThreads - 1];
+      for (int first = 0; first < chunk; first += kPlanThreads) {
+        const int i = first + tid;
+        int cls = kClasses;
+        SeqWork x = {};
+        if (i < chunk) {
+          int lo = 0, hi = kPlanThreads - 1;  // the first sequence whose end is past i
+          while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (s_end[mid] > i) {
+              hi = mid;
+            } else {
+              lo = mid + 1;
+            }
+          }
+          x.seq = base + lo;
+          x.tile = i - (lo > 0 ? s_end[lo - 1] : 0);
+          x.q0 = s_q0[lo];
+          x.q_len = s_q[lo];
+          x.k0 = s_k0[lo];
+          x.k_len = s_k[lo];
+          const int n0 = tile_blocks(p, x, x.tile * span), n1 = tile_blocks(p, x, x.tile * span + p.tok_tile);
+          x.je = max(n0, n1);
+          x.slot = -1;
+          x.ranges = 1;
+          x.cost = x.je * (n1 > 0 ? kCostBlock : kCostHalf) + kCostItem;
+          cls = (kClasses - 1) - static_cast<int>(static_cast<long long>(kClasses - 1) * x.je / most);
+        }
+        if (pass == 0) {
+          if (i < chunk) atomicAdd(&s_base[cls], 1);
+          continue;
+        }
+        // stable places: tiles of the same class in earlier warps, then in earlier lanes
+        for (int c = tid; c < kPlanThreads / 32 * kClasses; c += kPlanThreads) (&s_count[0][0])[c] = 0;
+        __syncthreads();
+        const unsigned peers = __match_any_sync(0xffffffffu, cls);
+        const int rank = __popc(peers & ((1u << lane) - 1));
+        if (rank == 0 && cls < kClasses) s_count[warp][cls] = __popc(peers);
+        __syncthreads();
+        for (int c = warp; c < kClasses; c += kPlanThreads / 32) {  // lane: a warp's count
+          const int n = s_count[lane][c];
+          int inc = n;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += up;
+          }
+          const int at = s_base[c];
+          s_count[lane][c] = at + inc - n;
+          __syncwarp();
+          if (lane == 31) s_base[c] = at + inc;
+        }
+        __syncthreads();
+        if (cls < kClasses) {
+          const int at = s_count[warp][cls] + rank;
+          if (at < p.max_tiles) plan_tiles(p)[at] = x;
+          work += x.cost;
+        }
+        __syncthreads();
+      }
+      total += chunk;
+      __syncthreads();
+    }
+    if (pass == 0) {  // counts -> first places
+      if (warp == 0) {
+        int run = 0;
+        for (int i = 0; i < kClasses; i += 32) {
+          const int c = s_base[i + lane];
+          int inc = c;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += up;
+          }
+          s_base[i + lane] = run + inc - c;
+          run += __shfl_sync(0xffffffffu, inc, 31);
+        }
+      }
+      __syncthreads();
+    }
+  }
+  total = min(total, p.max_tiles);
+  int entries = total, joins = 0;
+  if (p.max_slots > 0) {
+    long long all;
+    block_scan(work, s_warp64, all);
+    long long done = 0;
+    int slots = 0;
+    entries = 0;
+    for (int first = 0; first < total; first += kPlanThreads) {
+      const int i = first + tid;
+      SeqWork x = {};
+      if (i < total) x = plan_tiles(p)[i];
+      long long chunk;
+      const long long before = done + block_scan(static_cast<long long>(x.cost), s_warp64, chunk) - x.cost;
+      int n = 0;  // ranges
+      if (i < total) {
+        const long long range = (all - before) * p.kv_heads / (2 * ctas) + 1;
+        n = static_cast<int>(min((x.cost + range / 2) / range, static_cast<long long>(x.je / kMinRange)));
+        n = min(max(n, 1), 64);
+      }
+      int asked;
+      const int cut = n > 1 ? n : 0;
+      const int slot = slots + block_scan(cut, s_warp, asked) - cut;
+      slots += asked;  // past max_slots nothing more is cut
+      if (cut > 0 && slot + cut > p.max_slots) n = 1;
+      // entries and cut tiles up to this one
+      long long sums;
+      const long long mine = n + (n > 1 ? 1ll << 32 : 0);
+      const long long upto = block_scan(mine, s_warp64, sums) - mine;
+      const int at = entries + static_cast<int>(upto & 0xffffffff);
+      if (n == 1) plan_entries(p)[at] = x;
+      if (n > 1) {
+        plan_joins(p)[joins + static_cast<int>(upto >> 32)] = at;
+        const int len = x.je / n, extra = x.je - len * n;
+        SeqWork y = x;
+        y.je = 0;
+        y.ranges = n;
+        for (int k = 0; k < n; ++k) {
+          y.jb = y.je;
+          y.je += len + (k < extra ? 1 : 0);
+          y.slot = slot + k;
+          plan_entries(p)[at + k] = y;
+        }
+      }
+      done += chunk;
+      entries += static_cast<int>(sums & 0xffffffff);
+      joins += static_cast<int>(sums >> 32);
+    }
+  }
+  if (tid == 0) {
+    p.plan[0] = entries;
+    p.plan[1] = ctas;
+    p.plan[2] = joins;
+  }
+}
+
 template <int HD, int DT, bool PAGED>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     flash_seq_tcgen05(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -156,33 +453,47 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   using C = SeqCfg<HD>;
   constexpr int KS = C::kStages;
   constexpr int NS = C::kNS;
+  constexpr int NQ = C::kNQ;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
-  uint64_t* q_full = bars;
-  uint64_t* v_tail = q_full + 1;  // the copy of a sequence's last, partial V block
+  uint64_t* item_full = bars;
+  uint64_t* item_empty = item_full + 2;
+  uint64_t* s_done = item_empty + 2;  // every S of the item has been formed
+  uint64_t* q_full = s_done + 2;
+  uint64_t* q_empty = q_full + NQ;
+  uint64_t* v_tail = q_empty + NQ;  // the copy of a sequence's last, partial V block
   uint64_t* k_full = v_tail + 1;
   uint64_t* k_empty = k_full + KS;
   uint64_t* v_full = k_empty + KS;
   uint64_t* v_empty = v_full + KS;
   uint64_t* s_full = v_empty + KS;
   uint64_t* p_full = s_full + NS;
-  uint64_t* turn = p_full + 4;
+  uint64_t* turn = p_full + NS;
   uint64_t* drain = turn + 2;
   uint64_t* pv_done = drain + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + NS);
-  __shared__ SeqWork s_work;
+  __shared__ SeqWork s_item[2];
+  __shared__ SeqOut s_out;  // read where it is used: kept out of the softmax loop's registers
 
   const int warp = warp_id();
   const int lane = lane_id();
-  const int kvh = blockIdx.y;
-  const int split = blockIdx.z;
 
   if (warp == 0 && lane == 0) {
     tma_prefetch_map(&tmQ);
     tma_prefetch_map(&tmK);
     tma_prefetch_map(&tmV);
-    mbar_init(q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 11);  // warps 1 to 3 and 4 to 11
+      mbar_init(&s_done[i], 1);
+      mbar_init(&turn[i], 128);
+      mbar_init(&drain[i], 1);
+    }
+    for (int i = 0; i < NQ; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
     mbar_init(v_tail, 1);
     for (int s = 0; s < KS; ++s) {
       mbar_init(&k_full[s], 1);
@@ -192,77 +503,70 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
       mbar_init(&pv_done[i], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 128);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&turn[i], 128);
-      mbar_init(&drain[i], 1);
-    }
     fence_mbar_init();
+    s_out = p.o;
   }
+  // item i of the plan
+  auto listed_item = [&](int i, int items) {
+    SeqWork x = {};
+    x.seq = -1;
+    if (i < items) {
+      const int e = i / p.kv_heads;
+      x = plan_entries(p)[e];
+      x.kvh = i - e * p.kv_heads;
+    }
+    return x;
+  };
+  // (up to here, and warps other than 3 up to the barrier, only this CTA's
+  // shared memory and TMEM are touched)
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
-  }
-  // everything above touched only this CTA's shared memory and TMEM
-  pdl_wait();
-  pdl_trigger();
-  if (warp == 3) {
-    // later tiles of a causal sequence see more keys: hand them out first
-    const SeqWork w = find_tile<PAGED>(p, static_cast<int>(gridDim.x - 1 - blockIdx.x));
-    if (lane == 0) s_work = w;
+  } else if (warp == 3) {
+    pdl_wait();
+    SeqWork w;
+    if (p.plan != nullptr) {
+      w = listed_item(blockIdx.x, p.plan[0] * p.kv_heads);
+    } else {
+      const int per = p.kv_heads * p.splits;
+      const int tile = blockIdx.x / per, rest = blockIdx.x - tile * per;
+      w = find_tile<PAGED>(p, tile);
+      const int range = rest / p.kv_heads;
+      w.kvh = rest - range * p.kv_heads;
+      const int t0 = w.tile * 2 * p.tok_tile;
+      const int n = max(tile_blocks(p, w, t0), tile_blocks(p, w, t0 + p.tok_tile));
+      const int len = (n + p.splits - 1) / p.splits;
+      w.jb = range * len;
+      w.je = w.jb + len;
+      w.slot = p.splits > 1 ? tile * p.splits + range : -1;
+    }
+    if (lane == 0) s_item[0] = w;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const SeqWork w = s_work;
-  const int tok0 = w.tile * 2 * p.tok_tile;  // first token of the CTA, within its sequence
-  const int shift = w.k_len - w.q_len;       // query i stands at key i + shift
-
-  // key blocks [jb, jb + nblk[t]) of each tile: this split's part
-  int nblk[kAttnTiles];
-  int nall = 0;
-#pragma unroll
-  for (int t = 0; t < kAttnTiles; ++t) {
-    const int t0 = tok0 + t * p.tok_tile;
-    int k_end = w.seq >= 0 && t0 < w.q_len ? w.k_len : 0;
-    if (p.causal && k_end > 0) k_end = min(k_end, min(t0 + p.tok_tile, w.q_len) + shift);
-    nblk[t] = k_end <= 0 ? 0 : (k_end + kAttnBN - 1) / kAttnBN;
-    nall = max(nall, nblk[t]);
-  }
-  const int per = (nall + p.splits - 1) / p.splits;
-  const int jb = split * per;
-#pragma unroll
-  for (int t = 0; t < kAttnTiles; ++t) nblk[t] = min(max(nblk[t] - jb, 0), per);
-  const int nmax = nblk[0] > nblk[1] ? nblk[0] : nblk[1];
-  const int nmin = nblk[0] < nblk[1] ? nblk[0] : nblk[1];
-  const int t_long = nblk[0] > nblk[1] ? 0 : 1;
-  const int n_pairs = nblk[0] + nblk[1];
+  pdl_wait();
+  pdl_trigger();
 
   // one K or V block: this lane's copy (a page or a part of one, or the
   // whole block of packed keys) and the bytes of all copies
-  auto boxes_of = [&](int j) {
-    if constexpr (PAGED) {
-      const int left = min(kAttnBN, w.k_len - (jb + j) * kAttnBN);
-      return (left + p.page_box - 1) / p.page_box;
-    } else {
-      return 1;
-    }
+  auto boxes_of = [&](const SeqWork& w, int key) {
+    return PAGED ? (min(kAttnBN, w.k_len - key) + p.page_box - 1) / p.page_box : 1;
   };
-  auto page_of = [&](int j) {
+  auto page_of = [&](const SeqWork& w, int key) {
     if constexpr (PAGED) {
-      if (j >= nmax || lane >= boxes_of(j)) return 0;
-      const int key = (jb + j) * kAttnBN + lane * p.page_box;
-      return p.page_table[w.seq * p.table_ld + (key >> p.page_shift)];
+      if (key >= w.k_len || lane >= boxes_of(w, key)) return 0;
+      return p.page_table[w.seq * p.table_ld + ((key + lane * p.page_box) >> p.page_shift)];
     } else {
       return 0;
     }
   };
-  auto load_block = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int j, int page) {
-    const int key = (jb + j) * kAttnBN;
-    const int n = boxes_of(j);
+  auto load_block = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, const SeqWork& w, int key, int page) {
+    const int n = boxes_of(w, key);
     const int rows = PAGED ? p.page_box : kAttnBN;
     if (lane == 0) mbar_arrive_expect_tx(bar, n * rows * HD * 2);
     __syncwarp();
@@ -279,57 +583,95 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
 #pragma unroll
       for (int c = 0; c < HD / 64; ++c)
-        tma_load_4d(dst + c * 16384 + lane * rows * 128, map, bar, c * 64, kvh, y, z);
+        tma_load_4d(dst + c * 16384 + lane * rows * 128, map, bar, c * 64, w.kvh, y, z);
     }
+  };
+  // item number `it` of this CTA, for the warps that do not draw items:
+  // false when a wait ran out
+  auto take_item = [&](int it, SeqWork& w, int code) {
+    if (!mbar_wait(&item_full[it & 1], (it >> 1) & 1, p.status, code)) return false;
+    w = s_item[it & 1];
+    return true;
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLow));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSeqRegsLow));
     if (warp == 0) {
-      if (nmax > 0) {
-        // ---------------- Q + K producer ----------------
+      // ---------------- items, Q and K ----------------
+      SeqWork w = s_item[0];
+      int kc = 0, qn = 0;  // K blocks and Q loads so far
+      for (int it = 0;; ++it) {
+        if (it >= 2 && !mbar_wait(&item_empty[it & 1], ((it >> 1) - 1) & 1, p.status, kDevTimeoutProducer)) break;
         if (lane == 0) {
-          const int tiles = nblk[1] > 0 ? 2 : 1;  // tile 1 has no keys when it has no tokens
-          const int first = nblk[0] > 0 ? 0 : 1;
-          mbar_arrive_expect_tx(q_full, (tiles - first) * p.tok_tile * p.group * HD * 2);
-          for (int t = first; t < tiles; ++t)
+          if (it > 0) s_item[it & 1] = w;
+          mbar_arrive(&item_full[it & 1]);
+        }
+        if (w.seq < 0) break;
+        // the next item's number, on its way while this one is fetched
+        int next = 0x7fffffff, items = 0;
+        if (p.plan != nullptr) {
+          items = p.plan[0] * p.kv_heads;
+          if (lane == 0) next = atomicAdd(p.plan + 1, 1);
+        }
+        const SeqBlocks g = seq_blocks(p, w);
+        const int n = g.most();
+        bool ok = true;
+        int key = w.jb * kAttnBN;
+        int page = n > 0 ? page_of(w, key) : 0;
+        for (int j = 0; j < n; ++j, ++kc, key += kAttnBN) {
+          const int s = kc % KS;
+          const int ahead = j + 1 < n ? page_of(w, key + kAttnBN) : 0;
+          if (!(ok = mbar_wait(&k_empty[s], ((kc / KS) & 1) ^ 1, p.status, kDevTimeoutProducer))) break;
+          load_block(smem + C::kKOff + s * C::kTileBytes, &tmK, &k_full[s], w, key, page);
+          page = ahead;
+          if (j == 0) {
+            const int qs = qn % NQ;
+            if (!(ok = mbar_wait(&q_empty[qs], ((qn / NQ) & 1) ^ 1, p.status, kDevTimeoutProducer))) break;
+            if (lane == 0) {
+              const int first = g.n0 > 0 ? 0 : 1, last = g.n1 > 0 ? 1 : 0;  // tiles with keys
+              mbar_arrive_expect_tx(&q_full[qs], (last - first + 1) * p.tok_tile * p.group * HD * 2);
+              for (int t = first; t <= last; ++t)
 #pragma unroll
-            for (int c = 0; c < HD / 64; ++c)
-              tma_load_4d(smem + C::kQOff + t * C::kTileBytes + c * 16384, &tmQ, q_full, c * 64, 0, kvh,
-                          w.q0 + tok0 + t * p.tok_tile);
+                for (int c = 0; c < HD / 64; ++c)
+                  tma_load_4d(smem + C::kQOff + (qs * kAttnTiles + t) * C::kTileBytes + c * 16384, &tmQ, &q_full[qs],
+                              c * 64, 0, w.kvh, w.q0 + g.tok0 + t * p.tok_tile);
+            }
+            ++qn;
+          }
         }
-        int page = page_of(0);
-        int j = 0;
-        for (; j < nmax; ++j) {
-          const int s = j % KS;
-          const int next = page_of(j + 1);
-          if (!mbar_wait(&k_empty[s], ((j / KS) & 1) ^ 1, p.status, kDevTimeoutProducer)) break;
-          load_block(smem + C::kKOff + s * C::kTileBytes, &tmK, &k_full[s], j, page);
-          page = next;
-        }
-        mbar_wait(q_full, 0, p.status, kDevTimeoutDrain);
-        for (int i = (j > KS ? j - KS : 0); i < j; ++i)
-          mbar_wait(&k_full[i % KS], (i / KS) & 1, p.status, kDevTimeoutDrain);
+        if (!ok) break;
+        w = listed_item(__shfl_sync(0xffffffffu, next, 0), items);
       }
+      for (int i = max(qn - NQ, 0); i < qn; ++i) mbar_wait(&q_full[i % NQ], (i / NQ) & 1, p.status, kDevTimeoutDrain);
+      for (int i = max(kc - KS, 0); i < kc; ++i) mbar_wait(&k_full[i % KS], (i / KS) & 1, p.status, kDevTimeoutDrain);
     } else if (warp == 2) {
-      if (nmax > 0) {
-        // ---------------- V producer ----------------
-        int page = page_of(0);
-        int j = 0;
-        for (; j < nmax; ++j) {
-          const int s = j % KS;
-          const int next = page_of(j + 1);
-          if (!mbar_wait(&v_empty[s], ((j / KS) & 1) ^ 1, p.status, kDevTimeoutProducer)) break;
+      // ---------------- V ----------------
+      SeqWork w;
+      int vc = 0, tails = 0;
+      for (int it = 0; take_item(it, w, kDevTimeoutProducer); ++it) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[it & 1]);
+        if (w.seq < 0) break;
+        const SeqBlocks g = seq_blocks(p, w);
+        const int n = g.most();
+        bool ok = true;
+        int key = w.jb * kAttnBN;
+        int page = n > 0 ? page_of(w, key) : 0;
+        for (int j = 0; j < n; ++j, ++vc, key += kAttnBN) {
+          const int s = vc % KS;
+          const int ahead = j + 1 < n ? page_of(w, key + kAttnBN) : 0;
+          if (!(ok = mbar_wait(&v_empty[s], ((vc / KS) & 1) ^ 1, p.status, kDevTimeoutProducer))) break;
           uint8_t* dst = smem + C::kVOff + s * C::kTileBytes;
-          const int valid = w.k_len - (jb + j) * kAttnBN;
+          const int valid = w.k_len - key;
           if (valid >= kAttnBN) {
-            load_block(dst, &tmV, &v_full[s], j, page);
+            load_block(dst, &tmV, &v_full[s], w, key, page);
           } else {
             // the sequence ends inside this block: rows from `valid` on hold
             // another sequence's values, an unused part of a page or what the
             // stage held before
-            load_block(dst, &tmV, v_tail, j, page);
-            if (!mbar_wait(v_tail, 0, p.status, kDevTimeoutProducer)) break;
+            load_block(dst, &tmV, v_tail, w, key, page);
+            if (!(ok = mbar_wait(v_tail, tails & 1, p.status, kDevTimeoutProducer))) break;
+            ++tails;
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c)
               for (int i = valid * 8 + lane; i < kAttnBN * 8; i += 32)
@@ -338,218 +680,282 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[s]);
           }
-          page = next;
+          page = ahead;
         }
-        for (int i = (j > KS ? j - KS : 0); i < j; ++i)
-          mbar_wait(&v_full[i % KS], (i / KS) & 1, p.status, kDevTimeoutDrain);
+        if (!ok) break;
       }
-    } else if (warp == 1 || warp == 3) {
-      if (lane == 0 && nmax > 0) {
-        // ---------------- MMA issuers: warp 1 S = Q K^T, warp 3 O += P V ----------------
+      for (int i = max(vc - KS, 0); i < vc; ++i) mbar_wait(&v_full[i % KS], (i / KS) & 1, p.status, kDevTimeoutDrain);
+    } else if (lane == 0) {
+      // ---------------- MMA issuers: warp 1 S = Q K^T, warp 3 O += P V ----------------
+      // Pairs (tile, block) in the order (0, j), (1, j), (0, j + 1), ... go
+      // round the NS slots; slots, stages and their phases are counted on, not
+      // computed: what these threads do between two products idles the tensor
+      // core.
+      const uint32_t sbase = smem_u32(smem);
+      SeqWork w;
+      int slot = 0, ks = 0;
+      uint32_t slot_ph = 0, ks_ph = 0;
+      if (warp == 1) {
         constexpr uint32_t idesc_s = idesc_16_f32(DT, kAttnBM, kAttnBN);
-        constexpr uint32_t idesc_o = idesc_16_f32(DT, kAttnBM, HD, false, true);
-        const uint32_t sbase = smem_u32(smem);
-        auto pair_of = [&](int q, int& t, int& j) {
-          if (q < 2 * nmin) {
-            j = q >> 1;
-            t = q & 1;
-          } else {
-            j = nmin + (q - 2 * nmin);
-            t = t_long;
-          }
-        };
-        auto last_user = [&](int t, int j) { return t == 1 || j >= nblk[1]; };
+        int qs = 0;
+        uint32_t q_ph = 0;
         bool ok = true;
-        if (warp == 1) {
-          ok = mbar_wait(q_full, 0, p.status, kDevTimeoutMma);
-          for (int q = 0; q < n_pairs && ok; ++q) {
-            int t, j;
-            pair_of(q, t, j);
-            const int slot = q % NS;
-            if (q >= NS && !(ok = mbar_wait(&pv_done[slot], ((q - NS) / NS) & 1, p.status, kDevTimeoutMma))) break;
-            if (!(ok = mbar_wait(&k_full[j % KS], (j / KS) & 1, p.status, kDevTimeoutMma))) break;
-            tc_fence_after();
-            const uint32_t qa = sbase + C::kQOff + t * C::kTileBytes;
-            const uint32_t ka = sbase + C::kKOff + (j % KS) * C::kTileBytes;
-#pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-              const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-              umma_f16_ss(tmem_base + C::kTmS + slot * 128, smem_desc_sw128(qa + off, 16, 1024),
-                          smem_desc_sw128(ka + off, 16, 1024), idesc_s, k > 0 ? 1u : 0u);
-            }
-            umma_commit(&s_full[slot]);
-            if (last_user(t, j)) umma_commit(&k_empty[j % KS]);
+        for (int it = 0; ok && take_item(it, w, kDevTimeoutMma); ++it) {
+          mbar_arrive(&item_empty[it & 1]);
+          if (w.seq < 0) break;
+          const SeqBlocks g = seq_blocks(p, w);
+          const int n = g.most();
+          if (n == 0) {
+            mbar_arrive(&s_done[it & 1]);
+            continue;
           }
-        } else {
-          for (int q = 0; q < n_pairs && ok; ++q) {
-            int t, j;
-            pair_of(q, t, j);
-            const int slot = q % NS;
-            if (!(ok = mbar_wait(&v_full[j % KS], (j / KS) & 1, p.status, kDevTimeoutMma))) break;
-            if (!(ok = mbar_wait(&p_full[t * 2 + (j & 1)], (j >> 1) & 1, p.status, kDevTimeoutMma))) break;
-            tc_fence_after();
-            const uint32_t va = sbase + C::kVOff + (j % KS) * C::kTileBytes;
+          ok = mbar_wait(&q_full[qs], q_ph, p.status, kDevTimeoutMma);
+          const uint32_t qa0 = sbase + C::kQOff + qs * (kAttnTiles * C::kTileBytes);
+          for (int j = 0; j < n && ok; ++j) {
+            if (!(ok = mbar_wait(&k_full[ks], ks_ph, p.status, kDevTimeoutMma))) break;
+            const uint32_t ka = sbase + C::kKOff + ks * C::kTileBytes;
 #pragma unroll
-            for (int k = 0; k < kAttnBN / 16; ++k)
-              umma_f16_ts(tmem_base + C::kTmO + t * HD, tmem_base + C::kTmS + slot * 128 + k * 8,
-                          smem_desc_sw128(va + k * 2048, 16384, 1024), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
-            umma_commit(&pv_done[slot]);
-            if (last_user(t, j)) umma_commit(&v_empty[j % KS]);
+            for (int t = 0; t < kAttnTiles; ++t) {
+              if (j >= (t == 0 ? g.n0 : g.n1)) continue;
+              // the PV that read this slot's last P
+              if (!(ok = mbar_wait(&pv_done[slot], slot_ph ^ 1u, p.status, kDevTimeoutMma))) break;
+              tc_fence_after();
+              const uint32_t qa = qa0 + t * C::kTileBytes;
+#pragma unroll
+              for (int k = 0; k < HD / 16; ++k) {
+                const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+                umma_f16_ss(tmem_base + C::kTmS + slot * 128, smem_desc_sw128(qa + off, 16, 1024),
+                            smem_desc_sw128(ka + off, 16, 1024), idesc_s, k > 0 ? 1u : 0u);
+              }
+              umma_commit(&s_full[slot]);
+              if (++slot == NS) {
+                slot = 0;
+                slot_ph ^= 1u;
+              }
+            }
+            umma_commit(&k_empty[ks]);
+            if (++ks == KS) {
+              ks = 0;
+              ks_ph ^= 1u;
+            }
+          }
+          umma_commit(&q_empty[qs]);
+          umma_commit(&s_done[it & 1]);
+          if (++qs == NQ) {
+            qs = 0;
+            q_ph ^= 1u;
           }
         }
-        uint64_t* d = &drain[warp == 1 ? 0 : 1];
-        umma_commit(d);
-        mbar_wait(d, 0, p.status, kDevTimeoutDrain);
+      } else {
+        constexpr uint32_t idesc_o = idesc_16_f32(DT, kAttnBM, HD, false, true);
+        bool ok = true;
+        for (int it = 0; ok && take_item(it, w, kDevTimeoutMma); ++it) {
+          mbar_arrive(&item_empty[it & 1]);
+          if (w.seq < 0) break;
+          const SeqBlocks g = seq_blocks(p, w);
+          const int n = g.most();
+          for (int j = 0; j < n && ok; ++j) {
+            if (!(ok = mbar_wait(&v_full[ks], ks_ph, p.status, kDevTimeoutMma))) break;
+            const uint32_t va = sbase + C::kVOff + ks * C::kTileBytes;
+#pragma unroll
+            for (int t = 0; t < kAttnTiles; ++t) {
+              if (j >= (t == 0 ? g.n0 : g.n1)) continue;
+              // (O of the tile's last item has been read: this P comes from the threads that read it)
+              if (!(ok = mbar_wait(&p_full[slot], slot_ph, p.status, kDevTimeoutMma))) break;
+              tc_fence_after();
+#pragma unroll
+              for (int k = 0; k < kAttnBN / 16; ++k)
+                umma_f16_ts(tmem_base + C::kTmO + t * HD, tmem_base + C::kTmS + slot * 128 + k * 8,
+                            smem_desc_sw128(va + k * 2048, 16384, 1024), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+              umma_commit(&pv_done[slot]);
+              if (++slot == NS) {
+                slot = 0;
+                slot_ph ^= 1u;
+              }
+            }
+            umma_commit(&v_empty[ks]);
+            if (++ks == KS) {
+              ks = 0;
+              ks_ph ^= 1u;
+            }
+          }
+        }
       }
+      // drain: every MMA this thread issued completes before TMEM is released
+      uint64_t* d = &drain[warp == 1 ? 0 : 1];
+      umma_commit(d);
+      mbar_wait(d, 0, p.status, kDevTimeoutDrain);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsHigh));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSeqRegsHigh));
     // ---------------- softmax (warps 4..11) ----------------
     const int t = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const int tl = r / p.group;  // token within the tile
-    const int tok = tok0 + t * p.tok_tile + tl;
-    const bool live = w.seq >= 0 && tl < p.tok_tile && tok < w.q_len;
-    // keys this row admits, from its first block on
-    const int admit = (p.causal ? min(w.k_len, tok + shift + 1) : w.k_len) - jb * kAttnBN;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tm_s = tmem_base + lane_off + C::kTmS;
     const uint32_t tm_o = tmem_base + lane_off + C::kTmO + t * HD;
-    const int nb = nblk[t];
     const float c = p.scale_log2;
+    int qc = 0;  // pairs so far
+    int tn = 0;  // blocks so far in which the tiles took turns
 
-    // issue order of (t, j)
-    auto pair_at = [&](int j) { return j < nmin ? 2 * j + t : 2 * nmin + (j - nmin); };
-    // every PV up to the tile's block j has landed in O. The slot's barrier is
-    // exact: S of this thread's newest pair waited for the PV NS pairs back,
-    // so no phase before the awaited one of that slot is open. (One barrier
-    // per tile would not do: with one tile alone its PVs run up to NS behind.)
-    auto wait_pv = [&](int j) {
-      const int q = pair_at(j);
-      return mbar_wait(&pv_done[q % NS], (q / NS) & 1, p.status, kDevTimeoutSoftmax);
-    };
-
-    float m_ref = -INFINITY;
-    float l = 0.f;
-    bool ok = true;
-
-    for (int j = 0; j < nb; ++j) {
-      const int q = pair_at(j);
-      const int slot = q % NS;
-      if (!(ok = mbar_wait(&s_full[slot], (q / NS) & 1, p.status, kDevTimeoutSoftmax))) break;
-      tc_fence_after();
-      float s[128];
+    for (int it = 0;; ++it) {
+      if (!mbar_wait(&item_full[it & 1], (it >> 1) & 1, p.status, kDevTimeoutSoftmax)) break;
+      const SeqWork* item = &s_item[it & 1];
+      int nb, nmin, admit, pairs;
+      bool live;
       {
-        uint32_t v[128];
-        tmem_ld128(tm_s + slot * 128, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 128; ++i) s[i] = __uint_as_float(v[i]);
+        const SeqWork w = *item;
+        if (w.seq < 0) break;
+        const SeqBlocks g = seq_blocks(p, w);
+        nb = t == 0 ? g.n0 : g.n1;
+        nmin = g.both();
+        pairs = g.n0 + g.n1;
+        const int tok = g.tok0 + t * p.tok_tile + tl;
+        live = tl < p.tok_tile && tok < w.q_len;
+        // keys this row admits, from its first block on
+        admit = (p.causal ? min(w.k_len, tok + g.shift + 1) : w.k_len) - w.jb * kAttnBN;
       }
-      const int lim = admit - j * kAttnBN;
-      if (__any_sync(0xffffffffu, lim < kAttnBN)) {
-#pragma unroll
-        for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : -INFINITY;
-      }
+      // slot and phase of the tile's next pair in issue order, and of its last
+      // one: when that pair's PV has completed, every PV of the tile so far has
+      // landed in O. The slot's barrier is exact: S of this thread's newest pair
+      // waited for the PV NS pairs back, so no phase before the awaited one of
+      // that slot is open. (One barrier per tile would not do: with one tile
+      // alone its PVs run up to NS behind.)
+      const int q0 = qc + (nmin > 0 ? t : 0);
+      int slot = q0 % NS, pv_slot = 0;
+      uint32_t slot_ph = (q0 / NS) & 1, pv_ph = 0;
+      auto wait_pv = [&] { return mbar_wait(&pv_done[pv_slot], pv_ph, p.status, kDevTimeoutSoftmax); };
 
-      float mx[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mx[k] = fmax3f(s[k], s[8 + k], s[16 + k]);
-#pragma unroll
-      for (int base = 24; base < 120; base += 16)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mx[k] = fmax3f(mx[k], s[base + k], s[base + 8 + k]);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mx[k] = fmaxf(mx[k], s[120 + k]);
-      mx[0] = fmax3f(mx[0], mx[1], mx[2]);
-      mx[3] = fmax3f(mx[3], mx[4], mx[5]);
-      mx[0] = fmax3f(mx[0], mx[3], fmaxf(mx[6], mx[7]));
-      const float m_row = mx[0] * c;
+      float m_ref = -INFINITY;
+      float l = 0.f;
+      bool ok = true;
 
-      // rows that are not stored have no vote: results must not depend on them
-      const bool need = live && m_row > m_ref + kRescaleThreshold;
-      if (j == 0) {
-        m_ref = m_row;
-      } else if (__any_sync(0xffffffffu, need)) {
-        const float m_new = fmaxf(m_ref, m_row);
-        const float alpha = m_ref == -INFINITY ? 0.f : ex2_f32(m_ref - m_new);
-        if (!(ok = wait_pv(j - 1))) break;
+      for (int j = 0; j < nb; ++j) {
+        if (!(ok = mbar_wait(&s_full[slot], slot_ph, p.status, kDevTimeoutSoftmax))) break;
         tc_fence_after();
-        rescale_o<HD>(tm_o, alpha);
-        l *= alpha;
-        m_ref = m_new;
-      }
-      const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-
-      uint32_t pk[64];
-      float ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        float s[128];
+        {
+          uint32_t v[128];
+          tmem_ld128(tm_s + slot * 128, v);
+          tmem_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 128; ++i) s[i] = fmaf(s[i], c, -m_use);
-      if (j < nmin && (t == 1 || j > 0)) {
-        const uint32_t par = t == 0 ? ((j - 1) & 1) : (j & 1);
-        if (!(ok = mbar_wait(&turn[t], par, p.status, kDevTimeoutSoftmax))) break;
-      }
+          for (int i = 0; i < 128; ++i) s[i] = __uint_as_float(v[i]);
+        }
+        const int lim = admit - j * kAttnBN;
+        if (__any_sync(0xffffffffu, lim < kAttnBN)) {
 #pragma unroll
-      for (int i = 0; i < 128; ++i) s[i] = ex2_f32(s[i]);
-      if (j < nmin) mbar_arrive(&turn[1 - t]);
+          for (int i = 0; i < 128; ++i) s[i] = i < lim ? s[i] : -INFINITY;
+        }
+
+        float mx[8];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        pk[i] = pack_p<DT>(s[2 * i], s[2 * i + 1]);
-        ls[i & 7] += s[2 * i] + s[2 * i + 1];
+        for (int k = 0; k < 8; ++k) mx[k] = fmax3f(s[k], s[8 + k], s[16 + k]);
+#pragma unroll
+        for (int base = 24; base < 120; base += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mx[k] = fmax3f(mx[k], s[base + k], s[base + 8 + k]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx[k] = fmaxf(mx[k], s[120 + k]);
+        mx[0] = fmax3f(mx[0], mx[1], mx[2]);
+        mx[3] = fmax3f(mx[3], mx[4], mx[5]);
+        mx[0] = fmax3f(mx[0], mx[3], fmaxf(mx[6], mx[7]));
+        const float m_row = mx[0] * c;
+
+        // rows that are not stored have no vote: results must not depend on them
+        const bool need = live && m_row > m_ref + kRescaleThreshold;
+        if (j == 0) {
+          m_ref = m_row;
+        } else if (__any_sync(0xffffffffu, need)) {
+          const float m_new = fmaxf(m_ref, m_row);
+          const float alpha = m_ref == -INFINITY ? 0.f : ex2_f32(m_ref - m_new);
+          if (!(ok = wait_pv())) break;
+          tc_fence_after();
+          rescale_o<HD>(tm_o, alpha);
+          l *= alpha;
+          m_ref = m_new;
+        }
+        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+
+        uint32_t pk[64];
+        float ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 128; ++i) s[i] = fmaf(s[i], c, -m_use);
+        // tile 1 of a block after tile 0, tile 0 after tile 1 of the block before
+        if (j < nmin && tn + j + t > 0) {
+          if (!(ok = mbar_wait(&turn[t], (tn + j + t - 1) & 1, p.status, kDevTimeoutSoftmax))) break;
+        }
+#pragma unroll
+        for (int i = 0; i < 128; ++i) s[i] = ex2_f32(s[i]);
+        if (j < nmin) mbar_arrive(&turn[1 - t]);
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+          pk[i] = pack_p<DT>(s[2 * i], s[2 * i + 1]);
+          ls[i & 7] += s[2 * i] + s[2 * i + 1];
+        }
+        l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+
+        tmem_st64(tm_s + slot * 128, pk);
+        tmem_wait_st_all();
+        tc_fence_before();
+        mbar_arrive(&p_full[slot]);
+        pv_slot = slot;
+        pv_ph = slot_ph;
+        slot += j + 1 < nmin ? 2 : j < nmin ? 2 - t : 1;
+        if (slot >= NS) {
+          slot -= NS;
+          slot_ph ^= 1u;
+        }
       }
-      l += ((ls[0] + ls[1]) + (ls[2] + ls[3])) + ((ls[4] + ls[5]) + (ls[6] + ls[7]));
+      if (!ok) break;
 
-      tmem_st64(tm_s + slot * 128, pk);
-      tmem_wait_st_all();
-      tc_fence_before();
-      mbar_arrive(&p_full[t * 2 + (j & 1)]);
-    }
-
-    // ---------------- epilogue ----------------
-    if (ok) {
+      // ---------------- epilogue ----------------
       uint32_t ov[HD];
       if (nb > 0) {
-        ok = wait_pv(nb - 1);
-        if (ok) {
-          tc_fence_after();
-          if constexpr (HD == 128) {
-            tmem_ld128(tm_o, ov);
-          } else {
-            tmem_ld64(tm_o, ov);
-          }
-          tmem_wait_ld();
+        if (!wait_pv()) break;
+        tc_fence_after();
+        if constexpr (HD == 128) {
+          tmem_ld128(tm_o, ov);
+        } else {
+          tmem_ld64(tm_o, ov);
         }
+        tmem_wait_ld();
+        tc_fence_before();
       } else {
 #pragma unroll
         for (int i = 0; i < HD; ++i) ov[i] = 0u;
       }
-      if (ok && live) {
+      qc += pairs;
+      tn += nmin;
+      if (live) {
         const float inv = l > 0.f ? 1.f / l : 0.f;
         const float lse = l > 0.f ? (m_ref + __log2f(l)) * 0.69314718055994531f : -INFINITY;
-        const long long token = w.q0 + tok;
-        const int head = kvh * p.group + (r - tl * p.group);
-        if (p.splits > 1) {
-          const long long at = (split * static_cast<long long>(p.tokens) + token) * p.heads + head;
-          p.lse_part[at] = lse;
+        const long long token = item->q0 + item->tile * 2 * p.tok_tile + t * p.tok_tile + tl;
+        const int head = item->kvh * p.group + (r - tl * p.group);
+        const SeqOut& o = s_out;
+        if (item->slot >= 0) {
+          const long long at =
+              (static_cast<long long>(item->slot) * p.kv_heads + item->kvh) * (kAttnTiles * kAttnBM) + t * kAttnBM + r;
+          o.lse_part[at] = lse;
           if (nb > 0) {
-            float4* dst = reinterpret_cast<float4*>(p.o_part + at * HD);
+            float4* dst = reinterpret_cast<float4*>(o.o_part + at * HD);
 #pragma unroll
             for (int i = 0; i < HD / 4; ++i)
               dst[i] = make_float4(__uint_as_float(ov[4 * i]) * inv, __uint_as_float(ov[4 * i + 1]) * inv,
                                    __uint_as_float(ov[4 * i + 2]) * inv, __uint_as_float(ov[4 * i + 3]) * inv);
           }
         } else {
-          if (p.lse != nullptr) p.lse[static_cast<long long>(head) * p.tokens + token] = lse;
-          const long long obase = token * p.o_ts + head * p.o_hs;
-          if (p.out_f32) {
-            float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + obase);
+          if (o.lse != nullptr) o.lse[static_cast<long long>(head) * o.tokens + token] = lse;
+          const long long obase = token * o.o_ts + head * o.o_hs;
+          if (o.out_f32) {
+            float4* dst = reinterpret_cast<float4*>(static_cast<float*>(o.out) + obase);
 #pragma unroll
             for (int i = 0; i < HD / 4; ++i)
               dst[i] = make_float4(__uint_as_float(ov[4 * i]) * inv, __uint_as_float(ov[4 * i + 1]) * inv,
                                    __uint_as_float(ov[4 * i + 2]) * inv, __uint_as_float(ov[4 * i + 3]) * inv);
           } else {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + obase);
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(o.out) + obase);
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i)
               dst[i] = make_uint4(
@@ -560,6 +966,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
         }
       }
+      // A tile without blocks in this item must not run ahead to the next
+      // item's slots: waiting there, it would take the phase before the last
+      // for the one to come. (Exact here: this item is released only below,
+      // so the barrier's next phase cannot have begun.)
+      if (!mbar_wait(&s_done[it & 1], (it >> 1) & 1, p.status, kDevTimeoutSoftmax)) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[it & 1]);
     }
   }
 
@@ -571,46 +984,72 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   }
 }
 
-// Joins the ranges of each (token, head): one warp per row, in range order.
-// Tokens outside the sequences are left alone.
-template <int HD, int DT>
+// Joins the ranges of each cut tile: blocks (cut tile, key head, 64 rows), one
+// warp per row at a time, in range order.
+template <int HD, int DT, bool PAGED>
 __global__ void __launch_bounds__(256) seq_combine_kernel(const __grid_constant__ SeqK p) {
+  constexpr int E = HD / 32;
+  __shared__ SeqWork s_item;
   pdl_wait();
   pdl_trigger();
-  constexpr int E = HD / 32;
-  const long long row = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5;
-  const int lane = lane_id();
-  if (row >= static_cast<long long>(p.tokens) * p.heads) return;
-  const long long token = row / p.heads;
-  const int head = static_cast<int>(row - token * p.heads);
-  if (token < p.cu_q[0] || token >= p.cu_q[p.batch]) return;
-  const long long stride = static_cast<long long>(p.tokens) * p.heads;
-  float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.lse_part[s * stride + row]);
-  float l = 0.f, acc[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) acc[i] = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float g = p.lse_part[s * stride + row];
-    if (g == -INFINITY) continue;  // a range without keys wrote no result
-    const float f = __expf(g - m);
-    l += f;
-    const float* src = p.o_part + (s * stride + row) * HD + lane * E;
-#pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = fmaf(f, src[i], acc[i]);
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const long long base = token * p.o_ts + head * p.o_hs + lane * E;
-#pragma unroll
-  for (int i = 0; i < E; i += 2) {
-    if (p.out_f32) {
-      *reinterpret_cast<float2*>(static_cast<float*>(p.out) + base + i) = make_float2(acc[i] * inv, acc[i + 1] * inv);
-    } else {
-      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + base + i) = pack2<DT>(acc[i] * inv, acc[i + 1] * inv);
+  const int lane = lane_id(), warp = threadIdx.x >> 5;
+  const int kvh = blockIdx.y;
+  if (warp == 0) {
+    SeqWork w = {};
+    w.seq = -1;
+    if (p.plan == nullptr) {
+      w = find_tile<PAGED>(p, blockIdx.x);
+      w.slot = blockIdx.x * p.splits;
+      w.ranges = p.splits;
+    } else if (static_cast<int>(blockIdx.x) < p.plan[2]) {
+      w = plan_entries(p)[plan_joins(p)[blockIdx.x]];
     }
+    if (lane == 0) s_item = w;
   }
-  if (p.lse != nullptr && lane == 0)
-    p.lse[static_cast<long long>(head) * p.tokens + token] = l > 0.f ? m + __logf(l) : -INFINITY;
+  __syncthreads();
+  const SeqWork w = s_item;
+  if (w.seq < 0) return;
+  const long long stride = static_cast<long long>(p.kv_heads) * (kAttnTiles * kAttnBM);  // from range to range
+  const long long first = (static_cast<long long>(w.slot) * p.kv_heads + kvh) * (kAttnTiles * kAttnBM);
+  for (int r = blockIdx.z * 64 + warp; r < (static_cast<int>(blockIdx.z) + 1) * 64; r += 8) {
+    const int t = r / kAttnBM, rr = r % kAttnBM;
+    const int tl = rr / p.group;
+    const int tok = w.tile * 2 * p.tok_tile + t * p.tok_tile + tl;
+    if (tl >= p.tok_tile || tok >= w.q_len) continue;
+    const float* lg = p.o.lse_part + first + r;
+    float m = -INFINITY;
+    for (int k = lane; k < w.ranges; k += 32) m = fmaxf(m, lg[k * stride]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    float l = 0.f, acc[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[i] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < w.ranges; ++k) {
+      const float x = lg[k * stride];
+      if (x == -INFINITY) continue;  // a range without keys wrote no result
+      const float f = __expf(x - m);
+      const float* src = p.o.o_part + (first + r + k * stride) * HD + lane * E;
+      l += f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) acc[i] = fmaf(f, src[i], acc[i]);
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const long long token = w.q0 + tok;
+    const int head = kvh * p.group + (rr - tl * p.group);
+    const long long base = token * p.o.o_ts + head * p.o.o_hs + lane * E;
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+      if (p.o.out_f32) {
+        *reinterpret_cast<float2*>(static_cast<float*>(p.o.out) + base + i) = make_float2(acc[i] * inv, acc[i + 1] * inv);
+      } else {
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.o.out) + base + i) =
+            pack2<DT>(acc[i] * inv, acc[i + 1] * inv);
+      }
+    }
+    if (p.o.lse != nullptr && lane == 0)
+      p.o.lse[static_cast<long long>(head) * p.o.tokens + token] = l > 0.f ? m + __logf(l) : -INFINITY;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -618,31 +1057,49 @@ __global__ void __launch_bounds__(256) seq_combine_kernel(const __grid_constant_
 // ---------------------------------------------------------------------------
 
 struct SeqPlan {
-  int tok_tile, tiles, splits;
+  int tok_tile, tiles, splits, ctas, slots;
+  bool listed;  // the tiles are listed by seq_plan_kernel
+  long long plan_bytes, bytes;
 };
 
-// Grid bound and key split of a call: every CTA tile of every sequence fits
-// the smaller of tokens / tile + batch and batch * (tiles of the longest).
-// Keys are split when that leaves SMs without a CTA, into ranges of at least
-// 4 key blocks (a shorter range costs more in start-up and joining than the
-// idle SMs it fills).
+// Grid bound and key cuts of a call: every CTA tile of every sequence fits the
+// smaller of tokens / tile + batch and batch * (tiles of the longest).
 SeqPlan plan_of(const SeqArgs& a) {
-  SeqPlan s;
+  SeqPlan s = {};
   s.tok_tile = kAttnBM / (a.heads / a.kv_heads);
   const long long span = 2 * s.tok_tile;
   const long long by_tokens = a.tokens / span + a.batch;
   const long long by_longest = (a.max_q + span - 1) / span * a.batch;
   s.tiles = static_cast<int>(by_tokens < by_longest ? by_tokens : by_longest);
-  const long long ctas = static_cast<long long>(s.tiles) * a.kv_heads;
+  const int sms = device_sm_count();
+  const long long items = static_cast<long long>(s.tiles) * a.kv_heads;
   const long long blocks = (a.max_k + kAttnBN - 1) / kAttnBN;
-  long long n = ctas > 0 ? device_sm_count() / ctas : 1;
-  if (n > blocks / 4) n = blocks / 4;
-  s.splits = n < 1 ? 1 : n > 64 ? 64 : static_cast<int>(n);
+  s.listed = items > sms;
+  s.splits = 1;
+  if (s.listed) {
+    // Cuts pay where one item is long against an SM's share of all of them:
+    // at 16 key blocks (25 us) and up to 16 items per SM. Their slots (four
+    // per SM) are split over the key heads.
+    s.slots = blocks >= 16 && items <= 16ll * sms ? 4 * sms / a.kv_heads / 2 * 2 : 0;
+  } else if (items > 0) {
+    // as many ranges per tile as fill the SMs, of at least 4 key blocks (a
+    // shorter range costs more in start-up and joining than the SMs it fills)
+    long long n = sms / items;
+    if (n > blocks / 4) n = blocks / 4;
+    s.splits = n < 1 ? 1 : n > 64 ? 64 : static_cast<int>(n);
+    s.slots = s.splits > 1 ? s.tiles * s.splits : 0;
+  }
+  s.ctas = static_cast<int>(s.listed ? sms : items * s.splits);
+  if (s.listed)
+    s.plan_bytes = (kPlanHead + s.slots / 2) * 4ll +
+                   sizeof(SeqWork) * (s.tiles + (s.slots > 0 ? static_cast<long long>(s.tiles) + s.slots : 0));
+  s.plan_bytes = (s.plan_bytes + 15) / 16 * 16;
+  s.bytes = s.plan_bytes + static_cast<long long>(s.slots) * a.kv_heads * (kAttnTiles * kAttnBM) * (a.head_dim + 1) * 4;
   return s;
 }
 
 template <int HD, int DT, bool PAGED>
-int launch_seq(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const SeqK& k, dim3 grid,
+int launch_seq(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const SeqK& k, int ctas,
                cudaStream_t stream) {
   using C = SeqCfg<HD>;
   auto kern = flash_seq_tcgen05<HD, DT, PAGED>;
@@ -661,11 +1118,13 @@ int launch_seq(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& 
     if (e != cudaSuccess) return set_error(TF_ERR_LAUNCH, "cudaFuncSetAttribute(flash_seq): %s", cudaGetErrorString(e));
     attr_done[dev & 63] = true;
   }
-  cudaError_t e = launch_k(kern, grid, dim3(kAttnThreads), C::kAlloc, stream, tq, tk, tv, k);
-  if (e == cudaSuccess && k.splits > 1) {
-    const long long rows = static_cast<long long>(k.tokens) * k.heads;
-    e = launch_k(seq_combine_kernel<HD, DT>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, stream, k);
-  }
+  cudaError_t e = cudaSuccess;
+  if (k.plan != nullptr) e = launch_k(seq_plan_kernel<PAGED>, dim3(1), dim3(kPlanThreads), 0, stream, k, ctas);
+  if (e == cudaSuccess) e = launch_k(kern, dim3(ctas), dim3(kAttnThreads), C::kAlloc, stream, tq, tk, tv, k);
+  const int joins = k.plan != nullptr ? k.max_slots / 2 : k.splits > 1 ? k.max_tiles : 0;
+  if (e == cudaSuccess && joins > 0)
+    e = launch_k(seq_combine_kernel<HD, DT, PAGED>, dim3(joins, k.kv_heads, kAttnTiles * kAttnBM / 64), dim3(256), 0,
+                 stream, k);
   if (e != cudaSuccess) return set_error(TF_ERR_LAUNCH, "flash_seq launch: %s", cudaGetErrorString(e));
   return TF_OK;
 }
@@ -709,8 +1168,7 @@ int seq_check(const SeqArgs& a, const char* fn) {
 long long seq_workspace(const SeqArgs& a) {
   if (a.batch <= 0 || a.tokens <= 0 || a.max_q <= 0) return 0;
   if (a.page_size > 0 && paged_is_decode(a)) return paged_decode_workspace(a);
-  const SeqPlan s = plan_of(a);
-  return s.splits > 1 ? a.tokens * a.heads * (a.head_dim + 1) * 4 * s.splits : 0;
+  return plan_of(a).bytes;
 }
 
 int seq_attention(const SeqArgs& args, cudaStream_t stream) {
@@ -732,10 +1190,10 @@ int seq_attention(const SeqArgs& args, cudaStream_t stream) {
   const SeqPlan plan = plan_of(a);
   const int group = a.heads / a.kv_heads;
   SeqK k = {};
-  k.out = a.out;
-  k.o_ts = a.o_ts;
-  k.o_hs = a.o_hs;
-  k.lse = a.lse;
+  k.o.out = a.out;
+  k.o.o_ts = a.o_ts;
+  k.o.o_hs = a.o_hs;
+  k.o.lse = a.lse;
   k.cu_q = a.cu_q;
   k.cu_k = a.cu_k;
   k.kv_lens = a.kv_lens;
@@ -749,11 +1207,16 @@ int seq_attention(const SeqArgs& args, cudaStream_t stream) {
   k.max_q = static_cast<int>(a.max_q < a.tokens ? a.max_q : a.tokens);
   k.tok_tile = plan.tok_tile;
   k.splits = plan.splits;
-  k.o_part = static_cast<float*>(a.workspace);
-  k.lse_part = k.o_part + a.tokens * a.heads * a.head_dim * plan.splits;
+  k.o.tokens = k.tokens;
+  k.kv_heads = a.kv_heads;
+  k.max_tiles = plan.tiles;
+  k.max_slots = plan.listed ? plan.slots : 0;
+  k.plan = plan.listed ? static_cast<int*>(a.workspace) : nullptr;
+  k.o.o_part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + plan.plan_bytes);
+  k.o.lse_part = k.o.o_part + static_cast<long long>(plan.slots) * a.kv_heads * (kAttnTiles * kAttnBM) * a.head_dim;
   k.scale_log2 = a.scale * 1.4426950408889634f;
   k.causal = a.causal;
-  k.out_f32 = a.out_f32;
+  k.o.out_f32 = a.out_f32;
   k.status = device_status_ptr();
   if (k.status == nullptr) return last_error_code();
 
@@ -774,13 +1237,12 @@ int seq_attention(const SeqArgs& args, cudaStream_t stream) {
     k.num_pages = static_cast<int>(a.num_pages);
     k.page_cap = a.max_pages * a.page_size;
   }
-  const dim3 grid(plan.tiles, a.kv_heads, plan.splits);
 #define TFB_SEQ(DT)                                                                                    \
   if (paged)                                                                                           \
-    return a.head_dim == 64 ? launch_seq<64, DT, true>(tq, tk, tv, k, grid, stream)                    \
-                            : launch_seq<128, DT, true>(tq, tk, tv, k, grid, stream);                  \
-  return a.head_dim == 64 ? launch_seq<64, DT, false>(tq, tk, tv, k, grid, stream)                     \
-                          : launch_seq<128, DT, false>(tq, tk, tv, k, grid, stream);
+    return a.head_dim == 64 ? launch_seq<64, DT, true>(tq, tk, tv, k, plan.ctas, stream)                    \
+                            : launch_seq<128, DT, true>(tq, tk, tv, k, plan.ctas, stream);                  \
+  return a.head_dim == 64 ? launch_seq<64, DT, false>(tq, tk, tv, k, plan.ctas, stream)                     \
+                          : launch_seq<128, DT, false>(tq, tk, tv, k, plan.ctas, stream);
   if (a.bf16) {
     TFB_SEQ(kDtBF16)
   }
