@@ -75,8 +75,8 @@ struct AttnCfg {
   static constexpr int kVOff = kKOff + kKStages * kTileBytes;
   static constexpr int kBarOff = kVOff + kVStages * kTileBytes;
   // q_full, k_full/empty[KS], v_full/empty[VS], s_full[NS],
-  // p_full[2 tiles x 2 alternating], turn[2], drain[2], pv_done[NS]
-  static constexpr int kNumBars = 1 + 2 * kKStages + 2 * kVStages + kNS + 4 + 2 + 2 + kNS;
+  // p_full[2 tiles x 4], turn[2], drain[2], pv_done[NS]
+  static constexpr int kNumBars = 1 + 2 * kKStages + 2 * kVStages + kNS + 8 + 2 + 2 + kNS;
   static constexpr int kBytes = kBarOff + kNumBars * 8 + 16;
   static constexpr int kAlloc = kBytes + 1024;
   // TMEM columns: S/P slots at 0, 128, ..; O_t at kNS*128 + t*HD (512 in all)
@@ -151,8 +151,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   uint64_t* v_empty = v_full + VS;
   constexpr int NS = C::kNS;
   uint64_t* s_full = v_empty + VS;
-  uint64_t* p_full = s_full + NS;  // [tile * 2 + (block & 1)]: alternating, so no waiter falls two phases behind
-  uint64_t* turn = p_full + 4;     // exp-phase hand-off between the two softmax warpgroups
+  uint64_t* p_full = s_full + NS;  // [tile * 4 + block % 4]: P(j) follows PV(j - NS), so no waiter falls two phases behind
+  uint64_t* turn = p_full + 8;     // exp-phase hand-off between the two softmax warpgroups
   uint64_t* drain = turn + 2;       // [issuer]: end-of-kernel drain of each MMA issuer
   uint64_t* pv_done = drain + 2;    // [slot]: the PV that read this slot's P has completed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + NS);
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(&v_empty[s], 1);
     }
     for (int i = 0; i < NS; ++i) mbar_init(&s_full[i], 1);
-    for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 128);
+    for (int i = 0; i < 8; ++i) mbar_init(&p_full[i], 128);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&turn[i], 128);
     }
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           pair_of(q, t, j);
           const int slot = q % NS;
           if (!(ok = mbar_wait(&v_full[j % VS], (j / VS) & 1, p.status, kDevTimeoutMma))) break;
-          if (!(ok = mbar_wait(&p_full[t * 2 + (j & 1)], (j >> 1) & 1, p.status, kDevTimeoutMma))) break;
+          if (!(ok = mbar_wait(&p_full[t * 4 + (j & 3)], (j >> 2) & 1, p.status, kDevTimeoutMma))) break;
           tc_fence_after();
           const uint32_t va = sbase + C::kVOff + (j % VS) * C::kTileBytes;
           // P: 128 keys = 64 TMEM columns, 8 per MMA; V: MN-major, 8-key
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       tmem_st64(tm_s + slot * 128, pk);
       tmem_wait_st_all();
       tc_fence_before();
-      mbar_arrive(&p_full[t * 2 + (j & 1)]);
+      mbar_arrive(&p_full[t * 4 + (j & 3)]);
     }
 
     // ---------------- epilogue ----------------
