@@ -142,6 +142,29 @@ def test_packed_listed(q_lens, k_lens, h, g, hd, causal):
         assert torch.equal(again, out) and torch.equal(lse2, lse)
 
 
+CUT = [  # more items than SMs, a few so long that their keys are cut into ranges
+    ([3] * 30 + [5], [100] * 30 + [9000], 16, 8, 64), ([130, 40, 2, 7] * 11, [9001, 60, 300, 7] + [150] * 40, 12, 4, 128),
+    ([300] * 6, [10000, 5, 300, 100, 8300, 0], 25, 25, 64), ([1, 2] * 600, [20, 1] * 599 + [12000, 6000], 4, 1, 128),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("q_lens,k_lens,h,g,hd", CUT)
+def test_long_among_short(q_lens, k_lens, h, g, hd, causal):
+    q, k, v, cu_q, cu_k = packed_case(q_lens, k_lens, h, g, hd, F16, peak=2.0)
+    args = (q, k, v, cu_q, cu_k, max(q_lens), hd ** -0.5)
+    out, lse = K.flash_attention_packed(*args, causal=causal, want_lse=True, max_k=max(k_lens))
+    check_packed(q, k, v, cu_q, cu_k, hd ** -0.5, causal, out, lse)
+    for _ in range(3):
+        again, lse2 = K.flash_attention_packed(*args, causal=causal, want_lse=True, max_k=max(k_lens))
+        assert torch.equal(again, out) and torch.equal(lse2, lse)
+    q, kc, vc, table, cu, lens, rows = paged_case(q_lens, k_lens, h, g, hd, 32, F16)
+    out, lse = K.flash_attention_paged(q, kc, vc, table, cu, lens, max(max(q_lens), 17), hd ** -0.5, causal=causal,
+                                       want_lse=True, max_kv=max(k_lens))
+    check_paged(q, rows, q_lens, hd ** -0.5, causal, out, lse)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("causal", [False, True])

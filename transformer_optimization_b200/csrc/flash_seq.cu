@@ -16,15 +16,18 @@
 //   the causal limit is per token and a tile spans fewer positions.
 // * More items (two tiles of a sequence, a key head) than SMs: seq_plan_kernel
 //   lists the tiles by falling number of key blocks and CTAs draw items from
-//   the list by a counter, so a long item never starts last. Fewer: CTA c takes
-//   item c, found by a warp scan over the lengths, and where keys are long
-//   every tile is cut into as many key ranges as fill the SMs. Either way the
-//   call needs no host copy of the lengths and keeps nothing, and cuts depend
-//   on sizes alone: results repeat bit for bit. (Cutting all work into one
-//   equal run per SM instead, at key blocks inside items, was slower: 16 ragged
-//   prompts 57 us against 46. SMs that are at different places in the code
-//   stall each other's instruction fetch, items in order of size keep them
-//   together.)
+//   the list by a counter, so a long item never starts last. Where the longest
+//   is longer than an SM's share of all and half of that again, long tiles are
+//   cut into key ranges of half a share (32 sequences of 5 tokens, 64 heads
+//   over 8, hd 128, one of 100 000 keys and the others of 1000: 158 us, uncut
+//   840). Fewer items: CTA c takes item c, found by a warp scan over the
+//   lengths, and where keys are long every tile is cut into as many ranges as
+//   fill the SMs. Either way the call needs no host copy of the lengths and
+//   keeps nothing, and cuts depend on lengths alone: results repeat bit for
+//   bit. (Cutting all work into one equal run per SM instead, at key blocks
+//   inside items, was slower: 16 ragged prompts 57 us against 46. SMs that are
+//   at different places in the code stall each other's instruction fetch,
+//   items in order of size keep them together.)
 // * The warps' rings and barriers run on from item to item, so the next item's
 //   Q, K and V arrive and its first scores are formed while the last one's
 //   softmax and stores still run (a CTA per item spent 5.5 us, hd 64, to
@@ -64,6 +67,7 @@ struct SeqWork {
   int slot;       // where a key range's result goes; -1: the range is all
   int kvh;        // key head
   int n0, n1;     // of the key blocks, those that each tile has
+  int ranges;     // of the tile
 };
 
 struct SeqK {
@@ -76,14 +80,14 @@ struct SeqK {
   int num_pages, page_shift, page_box;  // page_box: rows of a page one copy takes
   long long page_cap;                   // keys a page table row can hold
   int batch, heads, group, tokens, k_tokens, max_q;
-  int min_q;     // shorter sequences are another kernel's
   int tok_tile;  // tokens per 128-row tile
   float scale_log2;
   int causal;
   int kv_heads, max_tiles;
   int splits;       // without a list: key ranges per tile
-  int* plan;        // null, or 2 ints: tiles in the list, next item
-  SeqWork* list;    // with a plan: [max_tiles]; with splits: [tiles][kv_heads], for the join
+  int max_slots;    // with a list: key ranges (of all key heads together) that tiles may be cut into
+  int* plan;        // null, or: entries in the list, next item, cut tiles, 0, the cut tiles' first entries
+  SeqWork* list;    // with a plan: [max_tiles + max_slots]; with splits: [max_tiles], for the join
   int* status;
 };
 
@@ -125,7 +129,6 @@ __device__ __forceinline__ SeqWork seq_lens(const SeqK& p, int b, bool& bad) {
   w.q0 = min(max(c0, 0), p.tokens);
   w.q_len = min(min(max(c1, w.q0), p.tokens) - w.q0, p.max_q);
   bad = c0 < 0 || w.q_len != c1 - c0;
-  if (w.q_len < p.min_q) w.q_len = 0;
   if constexpr (PAGED) {
     const int kv = p.kv_lens[b];
     w.k0 = 0;
@@ -224,27 +227,43 @@ __device__ __forceinline__ int block_scan(int x, int* s_warp, int& total) {
 
 // Lists the call's tiles by falling number of key blocks (counting sort over
 // kClasses classes), and sets the item counter to the CTAs' first items. One
-// block. The order within a class depends on timing, results do not.
+// block. If tiles may be cut and the longest has half as many blocks again as an SM's
+// share of all, tiles longer than half that share become ranges of at most that: at
+// most 2 * total / range = 4 SMs' worth of them, which is what the workspace
+// holds. The order within a class depends on timing, results do not.
+constexpr int kMinRange = 6;    // key blocks; a shorter range costs more than it evens out
+constexpr int kCutBlocks = 64;  // key blocks a sequence may have from which on the call makes room for cuts
+
 template <bool PAGED>
 __global__ void __launch_bounds__(kPlanThreads) seq_plan_kernel(const __grid_constant__ SeqK p, int ctas) {
   __shared__ int s_q0[kPlanThreads], s_q[kPlanThreads], s_k0[kPlanThreads], s_k[kPlanThreads];
   __shared__ int s_end[kPlanThreads];  // tiles of the round's sequences up to each
-  __shared__ int s_place[kClasses];    // tiles of a class, then the place of its next
+  __shared__ int s_place[kClasses];    // entries of a class, then the place of its next
   __shared__ int s_warp[32];
-  __shared__ int s_most;
+  __shared__ int s_most, s_slots, s_joins;
+  __shared__ unsigned long long s_sum;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int span = 2 * p.tok_tile;
   if (tid < kClasses) s_place[tid] = 0;
-  if (tid == 0) s_most = 1;
+  if (tid == 0) {
+    s_most = 1;
+    s_slots = s_joins = 0;
+    s_sum = 0;
+  }
   pdl_wait();
   pdl_trigger();
   __syncthreads();
   int most = 1;
+  unsigned long long sum = 0;  // blocks, every tile taken as long as its sequence's last (no less than there are)
   for (int b = tid; b < p.batch; b += kPlanThreads) {
     bool bad;
     const SeqWork w = seq_lens<PAGED>(p, b, bad);
     if (bad) record_error(p.status, kDevBadIndex);
-    if (w.q_len > 0) most = max(most, tile_blocks(p, w, (w.q_len - 1) / p.tok_tile * p.tok_tile));
+    if (w.q_len > 0) {
+      const int last = tile_blocks(p, w, (w.q_len - 1) / p.tok_tile * p.tok_tile);
+      most = max(most, last);
+      sum += static_cast<unsigned long long>((w.q_len + span - 1) / span) * last;
+    }
     if (b < kPlanThreads) {
       s_q0[tid] = w.q0;
       s_q[tid] = w.q_len;
@@ -253,13 +272,50 @@ __global__ void __launch_bounds__(kPlanThreads) seq_plan_kernel(const __grid_con
     }
   }
   most = __reduce_max_sync(0xffffffffu, most);
-  if (lane == 0) atomicMax(&s_most, most);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) {
+    atomicMax(&s_most, most);
+    atomicAdd(&s_sum, sum);
+  }
   __syncthreads();
-  const float per_class = (kClasses - 1) / static_cast<float>(s_most);
-  int total = 0;  // tiles
-  // pass 0 counts the classes, pass 1 places the tiles
+  most = s_most;
+  int range = 0x7fffffff;
+  if (p.max_slots > 0) {
+    const unsigned long long share = s_sum * p.kv_heads / ctas + 1;
+    if (2 * most > 3 * share) range = max(static_cast<int>((share + 1) / 2), kMinRange);
+  }
+  const float per_class = (kClasses - 1) / static_cast<float>(min(most, range));
+
+  // tile i of the sequences in shared memory
+  auto tile_of = [&](int base, int i) {
+    int lo = 0, hi = kPlanThreads - 1;  // the first sequence whose end is past i
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (s_end[mid] > i) {
+        hi = mid;
+      } else {
+        lo = mid + 1;
+      }
+    }
+    SeqWork x = {};
+    x.seq = base + lo;
+    x.tile = i - (lo > 0 ? s_end[lo - 1] : 0);
+    x.q0 = s_q0[lo];
+    x.q_len = s_q[lo];
+    x.k0 = s_k0[lo];
+    x.k_len = s_k[lo];
+    x.je = 0x7fffffff;
+    set_blocks(p, x);
+    x.je = max(x.n0, x.n1);
+    x.slot = -1;
+    x.ranges = x.je > range ? (x.je + range - 1) / range : 1;
+    return x;
+  };
+  int entries = 0;
+  SeqWork kept = {};  // this thread's tile of the only round, from pass to pass
+  // pass 0 counts the classes, pass 1 places the entries
   for (int pass = 0; pass < 2; ++pass) {
-    total = 0;
     for (int base = 0; base < p.batch; base += kPlanThreads) {
       if (p.batch > kPlanThreads) {
         SeqWork w = {};
@@ -270,60 +326,69 @@ __global__ void __launch_bounds__(kPlanThreads) seq_plan_kernel(const __grid_con
         s_k0[tid] = w.k0;
         s_k[tid] = w.k_len;
       }
-      int round;
       if (pass == 0 || p.batch > kPlanThreads) {
         const int n = base + tid < p.batch ? (s_q[tid] + span - 1) / span : 0;
+        int round;
         s_end[tid] = block_scan(n, s_warp, round);
         __syncthreads();
       }
-      round = s_end[kPlanThreads - 1];
+      const int round = s_end[kPlanThreads - 1];
       for (int i = tid; i < round; i += kPlanThreads) {
-        int lo = 0, hi = kPlanThreads - 1;  // the first sequence whose end is past i
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (s_end[mid] > i) {
-            hi = mid;
-          } else {
-            lo = mid + 1;
-          }
+        const bool keep = p.batch <= kPlanThreads && i == tid;
+        SeqWork x = pass == 1 && keep ? kept : tile_of(base, i);
+        if (keep) kept = x;
+        const int len = (x.je + x.ranges - 1) / x.ranges;
+        const int cls = min(max(kClasses - 1 - static_cast<int>(len * per_class), 0), kClasses - 1);
+        int at = atomicAdd(&s_place[cls], x.ranges);
+        if (pass == 0) continue;
+        if (x.ranges == 1) {
+          if (at < p.max_tiles + p.max_slots) p.list[at] = x;
+          continue;
         }
-        SeqWork x = {};
-        x.seq = base + lo;
-        x.tile = i - (lo > 0 ? s_end[lo - 1] : 0);
-        x.q0 = s_q0[lo];
-        x.q_len = s_q[lo];
-        x.k0 = s_k0[lo];
-        x.k_len = s_k[lo];
-        x.je = 0x7fffffff;
-        x.slot = -1;
-        set_blocks(p, x);
-        const int blocks = max(x.n0, x.n1);
-        const int cls = min(max(kClasses - 1 - static_cast<int>(blocks * per_class), 0), kClasses - 1);
-        const int at = atomicAdd(&s_place[cls], 1);
-        if (pass == 1 && at < p.max_tiles) p.list[at] = x;
+        const int slot = atomicAdd(&s_slots, x.ranges);
+        const int join = atomicAdd(&s_joins, 1);
+        if (slot + x.ranges > p.max_slots || at + x.ranges > p.max_tiles + p.max_slots) {
+          record_error(p.status, kDevBadIndex);  // (cannot be: see above)
+          continue;
+        }
+        p.plan[4 + join] = at;
+        const int all = x.je;
+        x.je = 0;
+        for (int k = 0; k < x.ranges; ++k, ++at) {
+          x.jb = x.je;
+          x.je = min(x.jb + len, all);
+          x.slot = slot + k;
+          set_blocks(p, x);
+          p.list[at] = x;
+        }
       }
-      total += round;
       __syncthreads();
     }
-    if (pass == 0 && warp == 0) {  // counts -> first places
-      int run = 0;
-      for (int i = 0; i < kClasses; i += 32) {
-        const int c = s_place[i + lane];
-        int inc = c;
+    if (pass == 0) {
+      if (warp == 0) {  // counts -> first places
+        int run = 0;
+        for (int i = 0; i < kClasses; i += 32) {
+          const int c = s_place[i + lane];
+          int inc = c;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int up = __shfl_up_sync(0xffffffffu, inc, d);
-          if (lane >= d) inc += up;
+          for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += up;
+          }
+          s_place[i + lane] = run + inc - c;
+          run += __shfl_sync(0xffffffffu, inc, 31);
         }
-        s_place[i + lane] = run + inc - c;
-        run += __shfl_sync(0xffffffffu, inc, 31);
+        if (lane == 0) s_warp[0] = run;
       }
+      __syncthreads();
+      entries = s_warp[0];
+      __syncthreads();
     }
-    __syncthreads();
   }
   if (tid == 0) {
-    p.plan[0] = min(total, p.max_tiles);
+    p.plan[0] = min(entries, p.max_tiles + p.max_slots);
     p.plan[1] = ctas;
+    p.plan[2] = min(s_joins, p.max_slots / 2);
   }
 }
 
@@ -411,6 +476,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int tile = i / p.kv_heads;
       x = p.list[tile];
       x.kvh = i - tile * p.kv_heads;
+      if (x.slot >= 0) x.slot = x.slot * p.kv_heads + x.kvh;
     }
     return x;
   };
@@ -438,9 +504,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const int len = (max(w.n0, w.n1) + p.splits - 1) / p.splits;
         w.jb = range * len;
         w.je = w.jb + len;
-        w.slot = (tile * p.kv_heads + w.kvh) * p.splits + range;
+        w.slot = (tile * p.splits + range) * p.kv_heads + w.kvh;
+        w.ranges = p.splits;
         set_blocks(p, w);
-        if (lane == 0 && range == 0) p.list[tile * p.kv_heads + w.kvh] = w;
+        if (lane == 0 && range == 0 && w.kvh == 0) p.list[tile] = w;
       }
     }
     if (lane == 0) s_item[0] = w;
@@ -896,66 +963,76 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   }
 }
 
-// Joins a tile's key ranges, in order: blocks (tile and key head, 64 rows), a
+// Joins a tile's key ranges, in order: blocks take (tile, key head, 64 rows), a
 // thread per row and quarter of the columns. Four ranges' results are
-// requested at a time.
+// requested at a time. How many tiles were cut is on the device, often none:
+// the grid is kCombineCtas per SM and runs over what there is.
+constexpr int kCombineCtas = 4;
+
 template <int HD, int DT>
 __global__ void __launch_bounds__(256) seq_combine_kernel(const __grid_constant__ SeqK p) {
   constexpr int CH = HD / 16;  // float4 columns per thread
   constexpr int kRows = kAttnTiles * kAttnBM;
   pdl_wait();
   pdl_trigger();
-  const SeqWork w = p.list[blockIdx.x];
-  if (w.seq < 0) return;
-  const int r = blockIdx.y * 64 + (threadIdx.x & 63);
-  const int quarter = threadIdx.x >> 6;
-  const int t = r / kAttnBM, rr = r % kAttnBM;
-  const int tl = rr / p.group;
-  const int tok = (2 * w.tile + t) * p.tok_tile + tl;
-  if (tl >= p.tok_tile || tok >= w.q_len) return;
-  const float* lg = p.o.lse_part + static_cast<long long>(w.slot) * kRows + r;
-  const float4* part = reinterpret_cast<const float4*>(p.o.o_part) +
-                       (w.slot * static_cast<long long>(HD / 4) + quarter * CH) * kRows + r;
-  float m = -INFINITY;
+  const int items = (p.plan != nullptr ? p.plan[2] : p.max_tiles) * p.kv_heads * (kRows / 64);
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const int head_item = item / (kRows / 64), tile = head_item / p.kv_heads, kvh = head_item - tile * p.kv_heads;
+    const SeqWork w = p.list[p.plan != nullptr ? p.plan[4 + tile] : tile];
+    if (w.seq < 0) continue;
+    // ranges are kv_heads slots apart; the first is head 0's (list: counted in tiles)
+    const long long slot = p.plan != nullptr ? static_cast<long long>(w.slot) * p.kv_heads + kvh : w.slot + kvh;
+    const long long apart = static_cast<long long>(p.kv_heads) * kRows;
+    const int r = item % (kRows / 64) * 64 + (threadIdx.x & 63);
+    const int quarter = threadIdx.x >> 6;
+    const int t = r / kAttnBM, rr = r % kAttnBM;
+    const int tl = rr / p.group;
+    const int tok = (2 * w.tile + t) * p.tok_tile + tl;
+    if (tl >= p.tok_tile || tok >= w.q_len) continue;
+    const float* lg = p.o.lse_part + slot * kRows + r;
+    const float4* part =
+        reinterpret_cast<const float4*>(p.o.o_part) + (slot * (HD / 4) + quarter * CH) * kRows + r;
+    float m = -INFINITY;
 #pragma unroll 8
-  for (int k = 0; k < p.splits; ++k) m = fmaxf(m, lg[k * kRows]);
-  float l = 0.f;
-  float4 acc[CH];
+    for (int k = 0; k < w.ranges; ++k) m = fmaxf(m, lg[k * apart]);
+    float l = 0.f;
+    float4 acc[CH];
 #pragma unroll
-  for (int i = 0; i < CH; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < CH; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int k = 0; k < p.splits; ++k) {
-    const float x = lg[k * kRows];
-    if (x == -INFINITY) continue;  // without keys for this row: no result was written
-    const float f = __expf(x - m);
-    l += f;
+    for (int k = 0; k < w.ranges; ++k) {
+      const float x = lg[k * apart];
+      if (x == -INFINITY) continue;  // without keys for this row: no result was written
+      const float f = __expf(x - m);
+      l += f;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const float4 y = part[k * static_cast<long long>(HD / 4 * kRows) + i * kRows];
-      acc[i].x = fmaf(f, y.x, acc[i].x);
-      acc[i].y = fmaf(f, y.y, acc[i].y);
-      acc[i].z = fmaf(f, y.z, acc[i].z);
-      acc[i].w = fmaf(f, y.w, acc[i].w);
+      for (int i = 0; i < CH; ++i) {
+        const float4 y = part[k * apart * (HD / 4) + i * kRows];
+        acc[i].x = fmaf(f, y.x, acc[i].x);
+        acc[i].y = fmaf(f, y.y, acc[i].y);
+        acc[i].z = fmaf(f, y.z, acc[i].z);
+        acc[i].w = fmaf(f, y.w, acc[i].w);
+      }
     }
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const long long token = w.q0 + tok;
-  const int head = w.kvh * p.group + (rr - tl * p.group);
-  const long long base = token * p.o.o_ts + head * p.o.o_hs + quarter * (HD / 4);
-  if (p.o.out_f32) {
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const long long token = w.q0 + tok;
+    const int head = kvh * p.group + (rr - tl * p.group);
+    const long long base = token * p.o.o_ts + head * p.o.o_hs + quarter * (HD / 4);
+    if (p.o.out_f32) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
-      reinterpret_cast<float4*>(static_cast<float*>(p.o.out) + base)[i] =
-          make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
-  } else {
+      for (int i = 0; i < CH; ++i)
+        reinterpret_cast<float4*>(static_cast<float*>(p.o.out) + base)[i] =
+            make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
+    } else {
 #pragma unroll
-    for (int i = 0; i < CH; i += 2)
-      reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o.out) + base)[i / 2] =
-          make_uint4(pack2<DT>(acc[i].x * inv, acc[i].y * inv), pack2<DT>(acc[i].z * inv, acc[i].w * inv),
-                     pack2<DT>(acc[i + 1].x * inv, acc[i + 1].y * inv), pack2<DT>(acc[i + 1].z * inv, acc[i + 1].w * inv));
+      for (int i = 0; i < CH; i += 2)
+        reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o.out) + base)[i / 2] =
+            make_uint4(pack2<DT>(acc[i].x * inv, acc[i].y * inv), pack2<DT>(acc[i].z * inv, acc[i].w * inv),
+                       pack2<DT>(acc[i + 1].x * inv, acc[i + 1].y * inv), pack2<DT>(acc[i + 1].z * inv, acc[i + 1].w * inv));
+    }
+    if (p.o.lse != nullptr && quarter == 0)
+      p.o.lse[static_cast<long long>(head) * p.o.tokens + token] = l > 0.f ? m + __logf(l) : -INFINITY;
   }
-  if (p.o.lse != nullptr && quarter == 0)
-    p.o.lse[static_cast<long long>(head) * p.o.tokens + token] = l > 0.f ? m + __logf(l) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -963,7 +1040,7 @@ __global__ void __launch_bounds__(256) seq_combine_kernel(const __grid_constant_
 // ---------------------------------------------------------------------------
 
 struct SeqPlan {
-  int tok_tile, tiles, splits, ctas;
+  int tok_tile, tiles, splits, ctas, slots;
   bool listed;  // the tiles are listed by seq_plan_kernel
   long long list_bytes, bytes;
 };
@@ -991,12 +1068,16 @@ SeqPlan plan_of(const SeqArgs& a) {
   }
   s.ctas = static_cast<int>(s.listed ? sms : items * s.splits);
   if (s.listed) {
-    s.list_bytes = 16 + s.tiles * static_cast<long long>(sizeof(SeqWork));
-    s.bytes = s.list_bytes;
+    const long long blocks = (a.max_k + kAttnBN - 1) / kAttnBN;
+    s.slots = blocks >= kCutBlocks ? 4 * sms / a.kv_heads : 0;
+    s.list_bytes = 16 + (s.slots / 2 * 4 + 15) / 16 * 16 +
+                   (s.tiles + static_cast<long long>(s.slots)) * static_cast<long long>(sizeof(SeqWork));
   } else if (s.splits > 1) {
-    s.list_bytes = (items * static_cast<long long>(sizeof(SeqWork)) + 15) / 16 * 16;
-    s.bytes = s.list_bytes + items * s.splits * (kAttnTiles * kAttnBM) * (a.head_dim + 1ll) * 4;
+    s.slots = s.tiles * s.splits;
+    s.list_bytes = s.tiles * static_cast<long long>(sizeof(SeqWork));
   }
+  s.list_bytes = (s.list_bytes + 15) / 16 * 16;
+  s.bytes = s.list_bytes + static_cast<long long>(s.slots) * a.kv_heads * (kAttnTiles * kAttnBM) * (a.head_dim + 1) * 4;
   return s;
 }
 
@@ -1023,9 +1104,12 @@ int launch_seq(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& 
   cudaError_t e = cudaSuccess;
   if (k.plan != nullptr) e = launch_k(seq_plan_kernel<PAGED>, dim3(1), dim3(kPlanThreads), 0, stream, k, ctas);
   if (e == cudaSuccess) e = launch_k(kern, dim3(ctas), dim3(kAttnThreads), C::kAlloc, stream, tq, tk, tv, k);
-  if (e == cudaSuccess && k.splits > 1)
-    e = launch_k(seq_combine_kernel<HD, DT>, dim3(k.max_tiles * k.kv_heads, kAttnTiles * kAttnBM / 64), dim3(256), 0,
+  const int joins = k.plan != nullptr ? k.max_slots / 2 : k.splits > 1 ? k.max_tiles : 0;  // at most
+  if (e == cudaSuccess && joins > 0) {
+    const int blocks = joins * k.kv_heads * (kAttnTiles * kAttnBM / 64);
+    e = launch_k(seq_combine_kernel<HD, DT>, dim3(std::min(blocks, kCombineCtas * device_sm_count())), dim3(256), 0,
                  stream, k);
+  }
   if (e != cudaSuccess) return set_error(TF_ERR_LAUNCH, "flash_seq launch: %s", cudaGetErrorString(e));
   return TF_OK;
 }
@@ -1111,14 +1195,17 @@ int seq_attention(const SeqArgs& args, cudaStream_t stream) {
   k.max_tiles = plan.tiles;
   k.splits = plan.splits;
   k.o.tokens = k.tokens;
+  char* ws = static_cast<char*>(a.workspace);
   if (plan.listed) {
-    k.plan = static_cast<int*>(a.workspace);
-    k.list = reinterpret_cast<SeqWork*>(k.plan + 4);
+    k.max_slots = plan.slots;
+    k.plan = reinterpret_cast<int*>(ws);
+    k.list = reinterpret_cast<SeqWork*>(ws + 16 + (plan.slots / 2 * 4 + 15) / 16 * 16);
   } else if (plan.splits > 1) {
-    k.list = static_cast<SeqWork*>(a.workspace);
-    k.o.o_part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + plan.list_bytes);
-    k.o.lse_part = k.o.o_part + static_cast<long long>(plan.ctas) * (kAttnTiles * kAttnBM) * a.head_dim;
+    k.list = reinterpret_cast<SeqWork*>(ws);
   }
+  k.o.o_part = reinterpret_cast<float*>(ws + plan.list_bytes);
+  k.o.lse_part =
+      k.o.o_part + static_cast<long long>(plan.slots) * a.kv_heads * (kAttnTiles * kAttnBM) * a.head_dim;
   k.scale_log2 = a.scale * 1.4426950408889634f;
   k.causal = a.causal;
   k.o.out_f32 = a.out_f32;
