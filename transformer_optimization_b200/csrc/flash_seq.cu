@@ -109,8 +109,8 @@ struct SeqCfg {
   static constexpr int kStageOff = kVOff + kStages * kTileBytes;  // 4 KB per softmax warp for the stores
   static constexpr int kBarOff = kStageOff + 8 * 4096;
   // item_full/empty[2], s_done[2], q_full/empty[NQ], v_tail, k_full/empty, v_full/empty,
-  // s_full[NS], p_full[NS], drain[2], pv_done[NS]
-  static constexpr int kNumBars = 6 + 2 * kNQ + 1 + 4 * kStages + 3 * kNS + 2;
+  // s_full[NS], p_full[NS], drain[2], pv_done[NS], o_done[2]
+  static constexpr int kNumBars = 6 + 2 * kNQ + 1 + 4 * kStages + 3 * kNS + 4;
   static constexpr int kBytes = kBarOff + kNumBars * 8 + 16;
   static constexpr int kAlloc = kBytes + 1024;
   static constexpr uint32_t kTmS = 0;
@@ -432,7 +432,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   uint64_t* p_full = s_full + NS;
   uint64_t* drain = p_full + NS;
   uint64_t* pv_done = drain + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + NS);
+  uint64_t* o_done = pv_done + NS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
   __shared__ SeqWork s_item[2];
   __shared__ SeqOut s_out;  // read where it is used: kept out of the softmax loop's registers
 
@@ -448,6 +449,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(&item_empty[i], 11);  // warps 1 to 3 and 4 to 11
       mbar_init(&s_done[i], 1);
       mbar_init(&drain[i], 1);
+      mbar_init(&o_done[i], 1);
     }
     for (int i = 0; i < NQ; ++i) {
       mbar_init(&q_full[i], 1);
@@ -731,6 +733,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 umma_f16_ts(tmem_base + C::kTmO + t * HD, tmem_base + C::kTmS + slot * 128 + k * 8,
                             smem_desc_sw128(va + k * 2048, 16384, 1024), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
               umma_commit(&pv_done[slot]);
+              if (j + 1 == (t == 0 ? w.n0 : w.n1)) umma_commit(&o_done[t]);
               if (++slot == NS) {
                 slot = 0;
                 slot_ph ^= 1u;
@@ -761,6 +764,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const uint32_t tm_o = tmem_base + lane_off + C::kTmO + t * HD;
     const float c = p.scale_log2;
     int qc = 0;  // pairs so far
+    uint32_t o_ph = 0;
 
     for (int it = 0;; ++it) {
       if (!seq_wait(&item_full[it & 1], (it >> 1) & 1, p.status, kDevTimeoutSoftmax)) break;
@@ -779,10 +783,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       // slot and phase of the tile's next pair in issue order, and of its last
       // one: when that pair's PV has completed, every PV of the tile so far has
-      // landed in O. The slot's barrier is exact: S of this thread's newest pair
-      // waited for the PV NS pairs back, so no phase before the awaited one of
-      // that slot is open. (One barrier per tile would not do: with one tile
-      // alone its PVs run up to NS behind.)
+      // landed in O. Within the item the slot's barrier is exact: S of this
+      // thread's newest pair waited for the PV NS pairs back, so no phase before
+      // the awaited one is open, and the slot's next PV comes after this
+      // thread's next P. (A single barrier for all of a tile's PVs would not do:
+      // with one tile alone they run up to NS behind.) At the item's end the
+      // other tile's PVs may come round to the slot, so that wait is on o_done,
+      // which completes once per item in which the tile has keys.
       const int q0 = qc + (nmin > 0 ? t : 0);
       int slot = q0 % NS, pv_slot = 0;
       uint32_t slot_ph = (q0 / NS) & 1, pv_ph = 0;
@@ -868,7 +875,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // ---------------- epilogue ----------------
       uint32_t ov[HD];
       if (nb > 0) {
-        if (!wait_pv()) break;
+        if (!seq_wait(&o_done[t], o_ph, p.status, kDevTimeoutSoftmax)) break;
+        o_ph ^= 1u;
         tc_fence_after();
         if constexpr (HD == 128) {
           tmem_ld128(tm_o, ov);
