@@ -503,7 +503,7 @@ def _rotary_operands(name, q, k, positions, freqs):
 
 def _rotary_out(name, what, x, out):
     if out is None:
-        return x.new_empty(x.shape)
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
     _need_heads(name, what, out, x.dtype)
     if out.shape != x.shape:
         raise ValueError(f"{name}: {what} must have its input's shape")
@@ -589,14 +589,14 @@ def _seq_operands(name, q, kv_heads, cu_q, max_q, scale, out, out_dtype, lse, wa
     if out_dtype not in (q.dtype, torch.float32):
         raise ValueError(f"{name}: out_dtype must be q's type or fp32")
     if out is None:
-        out = q.new_empty(q.shape, dtype=out_dtype)
+        out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
     else:
         _need_heads(name, "out", out, out_dtype)
         if out.shape != q.shape:
             raise ValueError(f"{name}: out must have q's shape")
     if lse is None:
         if want_lse:
-            lse = q.new_empty((h, t), dtype=torch.float32)
+            lse = torch.empty(h, t, dtype=torch.float32, device=q.device)
     elif lse.dtype != torch.float32 or lse.shape != (h, t) or not lse.is_contiguous():
         raise ValueError(f"{name}: lse must be contiguous fp32 [heads, tokens]")
     flags = (_abi.TF_ATTN_OUT_F32 if out_dtype == torch.float32 else 0) | (
@@ -614,7 +614,7 @@ def _seq_workspace_bytes(dev: int, fn: str, *sizes: int) -> int:
 def _seq_workspace(name, fn, dev, like, workspace, *sizes):
     need = _seq_workspace_bytes(dev, fn, *sizes)
     if workspace is None:
-        return (like.new_empty(need, dtype=torch.uint8), need) if need else (None, 0)
+        return (torch.empty(need, dtype=torch.uint8, device=like.device), need) if need else (None, 0)
     if not workspace.is_contiguous() or workspace.get_device() != dev:
         raise ValueError(f"{name}: workspace must be contiguous, on the operands' device")
     size = workspace.numel() * workspace.element_size()

@@ -4,10 +4,13 @@
     python -m transformer_optimization_b200.microbench flash B H S HD [--causal]
     python -m transformer_optimization_b200.microbench ln    M D
     python -m transformer_optimization_b200.microbench merge B S H HD
+    python -m transformer_optimization_b200.microbench rotary T H KVH HD       (into a paged cache)
+    python -m transformer_optimization_b200.microbench packed B S H KVH HD [--causal]
+    python -m transformer_optimization_b200.microbench paged  B S H KVH HD [--new N]
 
 Prints one line: kernel, shape, mean time per launch (ms) and the achieved
 rate against its roofline unit (TFLOP/s for GEMM/attention, GB/s for
-LayerNorm). Inputs are seeded random; --iters launches are timed after
+LayerNorm, merge, rotary and paged; the last three in bf16). Inputs are seeded random; --iters launches are timed after
 --warmup untimed ones. Also the command used for the committed ncu captures
 (small cases, single kernel).
 """
@@ -54,10 +57,11 @@ def _time(fn, warmup, iters, min_warm_s=0.3, min_time_s=0.2):
 
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("kernel", choices=("gemm", "gemm_res", "flash", "ln", "merge"))
+    ap.add_argument("kernel", choices=("gemm", "gemm_res", "flash", "ln", "merge", "rotary", "packed", "paged"))
     ap.add_argument("dims", type=int, nargs="+")
     ap.add_argument("--gelu", action="store_true")
     ap.add_argument("--causal", action="store_true")
+    ap.add_argument("--new", type=int, default=1, help="paged: new tokens per sequence")
     ap.add_argument("--pure", action="store_true", help="ln: LayerNorm only (no residual delta, no x write)")
     ap.add_argument("--exp-f16x2", action="store_true", help="flash: packed fp16 exp2 path")
     ap.add_argument("--fma-exp", type=int, default=0, help="flash: pairs per row exponentiated on the FMA pipes")
@@ -114,6 +118,38 @@ def main(argv=None):
         ms = T(lambda: K.attn_merge(o_acc, lse_acc, o_part, lse_part, h, out16=out16))
         nbytes = bsz * s * d * (4 + 4 + 4 + 2) + bsz * h * s * 4 * 3  # o_acc r+w, o_part r, fp16 out; lse r, r, w
         print(f"merge B={bsz} S={s} H={h} hd={hd}: {ms:.4f} ms  {nbytes / (ms / 1e3) / 1e9:.1f} GB/s")
+    elif a.kernel == "rotary":
+        # queries turned, keys turned and values copied into a cache of 64-row pages
+        t, h, g, hd = a.dims
+        qkv = torch.randn(t, h + 2 * g, hd, device=dev, dtype=torch.bfloat16)
+        q, k, v = qkv[:, :h], qkv[:, h:h + g], qkv[:, h + g:]
+        kc, vc = (torch.empty(-(-t // 64), 64, g, hd, device=dev, dtype=torch.bfloat16) for _ in range(2))
+        pos = torch.arange(t, device=dev)
+        freqs, _ = K.rotary_freqs(hd, device=dev)
+        q_out = torch.empty(t, h, hd, device=dev, dtype=torch.bfloat16)
+        ms = T(lambda: K.rotary_append(q, k, v, pos, freqs, kc, vc, pos, q_out=q_out))
+        print(f"rotary T={t} H={h} KVH={g} hd={hd}: {ms:.4f} ms  {t * (h + 2 * g) * hd * 4 / (ms / 1e3) / 1e9:.1f} GB/s")
+    elif a.kernel == "packed":
+        bsz, s, h, g, hd = a.dims
+        q = torch.randn(bsz * s, h, hd, device=dev, dtype=torch.bfloat16)
+        k, v = (torch.randn(bsz * s, g, hd, device=dev, dtype=torch.bfloat16) for _ in range(2))
+        cu = torch.arange(bsz + 1, device=dev, dtype=torch.int32) * s
+        ms = T(lambda: K.flash_attention_packed(q, k, v, cu, cu, s, hd ** -0.5, max_k=s, causal=a.causal))
+        flops = 4.0 * bsz * s * s * h * hd * (0.5 if a.causal else 1.0)
+        print(f"packed B={bsz} S={s} H={h} KVH={g} hd={hd} causal={a.causal}: {ms:.4f} ms  "
+              f"{flops / (ms / 1e3) / 1e12:.1f} TFLOP/s")
+    elif a.kernel == "paged":
+        # --new tokens of each of B sequences over S cached rows in pages of 16
+        bsz, s, h, g, hd = a.dims
+        per = -(-s // 16)
+        kc, vc = (torch.randn(bsz * per, 16, g, hd, device=dev, dtype=torch.bfloat16) for _ in range(2))
+        table = torch.randperm(bsz * per, device=dev).to(torch.int32).view(bsz, per)
+        q = torch.randn(bsz * a.new, h, hd, device=dev, dtype=torch.bfloat16)
+        cu = torch.arange(bsz + 1, device=dev, dtype=torch.int32) * a.new
+        lens = torch.full((bsz,), s, device=dev, dtype=torch.int32)
+        ms = T(lambda: K.flash_attention_paged(q, kc, vc, table, cu, lens, a.new, hd ** -0.5, max_kv=s))
+        print(f"paged B={bsz} S={s} H={h} KVH={g} hd={hd} new={a.new}: {ms:.4f} ms  "
+              f"{bsz * s * g * hd * 4 / (ms / 1e3) / 1e9:.1f} GB/s of cache")
     else:
         m, d = a.dims
         x = torch.randn(m, d, device=dev)
