@@ -293,7 +293,8 @@ int tf_attn_merge(float* o_acc, float* lse_acc, const float* o_part, const float
  * the rotation in fp32, one rounding to the 16-bit type. q: token and head
  * strides q_ts, q_hs, unit inner stride; likewise q_out, k, k_out (heads and
  * kv_heads of them; either count may be 0). Outputs may be their inputs (in
- * place) but must not overlap them otherwise. positions int64 [tokens], any
+ * place) but must not overlap them otherwise, and no two rows of an output may
+ * overlap. positions int64 [tokens], any
  * sign (negated positions give the transpose); freqs fp64 [rot / 2].
  * head_dim 2 .. 256, rot even. Any strides and 2-byte alignment; multiples of
  * 8 elements and 16-byte bases are fastest.
@@ -336,7 +337,8 @@ int tf_rotary_append(const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int
  * sequence's queries and keys (max_k only sizes the key split). Lengths or
  * offsets outside the arrays, or queries past max_q, are cut to the bound and
  * set device code 108. head_dim 64 or 128; heads a multiple of kv_heads, at
- * most 128 times; scale > 0; bases 16-byte aligned, strides multiples of 8.
+ * most 128 times; scale > 0; bases 16-byte aligned, strides multiples of 8; no
+ * two rows of out may overlap, nor out and an operand.
  * workspace: tf_flash_packed_workspace bytes (the same sizes, tokens = q's
  * rows), 16-byte aligned; calls that overlap in time need their own.
  * Replaces the attention of the reference's fp16 path for ragged batches,

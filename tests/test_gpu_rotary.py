@@ -246,6 +246,28 @@ def test_rotary_abi_refuses_without_device():
         assert lib.tf_last_error()
 
 
+@pytest.mark.parametrize("at,value", [(4, 0), (4, 64), (5, 0), (5, 62), (10, 32), (11, 0)])
+def test_rotary_abi_refuses_overlapping_results(at, value):
+    """Rows of an output in one place would be written in any order; inputs may repeat (stride 0)."""
+    from transformer_optimization_b200 import _abi
+    lib = _abi.load()
+    args = [64, 0, 0, 64, 128, 64, 64, 0, 0, 64, 128, 64, 64, 64, 4, 2, 2, 64, 32, 1.0, 0, None]
+    args[at] = value
+    assert lib.tf_rotary(*args) == 1
+    assert b"overlap" in lib.tf_last_error()
+
+
+@pytest.mark.parametrize("at,value", [(16, 0), (16, 1024), (17, 64), (18, 0)])
+def test_rotary_append_abi_refuses_overlapping_cache(at, value):
+    from transformer_optimization_b200 import _abi
+    lib = _abi.load()
+    args = [64, 128, 64, 64, 128, 64, 64, 128, 64, 64, 128, 64, 64, 64, 64, 64, 2048, 128, 64, 3, 16, 64, 4, 2, 2, 64, 32,
+            1.0, 0, None]
+    args[at] = value
+    assert lib.tf_rotary_append(*args) == 1
+    assert b"overlap" in lib.tf_last_error()
+
+
 def test_rotary_freqs_scaling():
     from transformer_optimization_b200 import kernels as K
     f, m = K.rotary_freqs(64)

@@ -588,3 +588,22 @@ def test_seq_abi_refuses_without_device():
         assert lib.tf_flash_paged(*args) == code, (at, value)
     assert lib.tf_flash_packed_workspace(8, 2, 4, 3, 64, 4, 9) == -1
     assert lib.tf_flash_paged_workspace(8, -2, 4, 2, 64, 4, 9) == -1
+
+
+@pytest.mark.parametrize("at,value", [(11, 0), (11, 192), (12, 0), (12, 56), (11, 64)])
+def test_seq_abi_refuses_overlapping_results(at, value):
+    """Rows of out in one place would be written in any order."""
+    lib = _abi.load()
+    args = [64, 256, 64, 64, 128, 64, 64, 128, 64, 64, 64, 64, 256, 64, None, 8, 9, 2, 4, 2, 64, 4, 9, 0.125, 0, None, 0,
+            None]
+    args[at + 1] = value
+    assert lib.tf_flash_packed(*args) == 1
+    assert b"overlap" in lib.tf_last_error()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_decode_workspace_needs_sizes_alone(hd):
+    """(on a host without a device the size cannot be known: -1, with the device's message, not a refusal of sizes)"""
+    lib = _abi.load()
+    need = lib.tf_flash_paged_workspace(8, 2, 4, 2, hd, 4, 9)
+    assert need > 0 or (not torch.cuda.is_available() and b"overlap" not in lib.tf_last_error())

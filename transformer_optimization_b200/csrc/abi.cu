@@ -649,8 +649,10 @@ static int64_t seq_workspace_common(const char* fn, int64_t tokens, int64_t batc
   a.max_k = max_k;
   a.page_size = page_size;
   a.scale = 1.f;
-  a.q = a.k = a.v = &a;  // sizes only: the pointer checks see an aligned stand-in
+  a.q = a.k = a.v = &a;  // sizes only: the pointer and stride checks see a dense, aligned stand-in
   a.out = &a;
+  a.o_hs = head_dim;
+  a.o_ts = head_dim * heads;
   a.cu_q = a.cu_k = a.kv_lens = reinterpret_cast<const int*>(&a);
   if (tfb::seq_check(a, fn)) return -1;
   if (begin_call()) return -1;

@@ -1233,6 +1233,8 @@ int seq_check(const SeqArgs& a, const char* fn) {
     return set_error(TF_ERR_ALIGN, "%s: q, keys, values, out and workspace must be 16-byte aligned", fn);
   for (long long s : {a.q_ts, a.q_hs, a.k_ts, a.k_hs, a.v_ts, a.v_hs, a.o_ts, a.o_hs, a.k_ps, a.v_ps})
     if (s < 0 || s % 8) return set_error(TF_ERR_ALIGN, "%s: strides must be multiples of 8 elements", fn);
+  if (!rows_apart(a.head_dim, {{a.o_ts, a.tokens}, {a.o_hs, a.heads}}))
+    return set_error(TF_ERR_SHAPE, "%s: rows of out overlap", fn);
   return TF_OK;
 }
 

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <utility>
 
 #include "../../include/tfb200.h"
@@ -23,6 +24,21 @@ int set_error(int code, const char* fmt, ...);
 int last_error_code();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Whether rows of `width` elements on axes (pitch, entries) lie apart: each
+// axis, from the smallest pitch up, steps over what the ones below span. Asked
+// of outputs: two rows in one place would be written in any order.
+template <int N>
+bool rows_apart(long long width, std::pair<long long, long long> (&&axes)[N]) {
+  std::sort(axes, axes + N);
+  long long span = width;
+  for (const auto& [pitch, entries] : axes) {
+    if (entries <= 1) continue;
+    if (pitch < span) return false;
+    span += (entries - 1) * pitch;
+  }
+  return true;
+}
 
 // Streaming-multiprocessor count of the current device (cached).
 int device_sm_count();
