@@ -503,7 +503,7 @@ def _rotary_operands(name, q, k, positions, freqs):
 
 def _rotary_out(name, what, x, out):
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
     _need_heads(name, what, out, x.dtype)
     if out.shape != x.shape:
         raise ValueError(f"{name}: {what} must have its input's shape")
@@ -589,7 +589,7 @@ def _seq_operands(name, q, kv_heads, cu_q, max_q, scale, out, out_dtype, lse, wa
     if out_dtype not in (q.dtype, torch.float32):
         raise ValueError(f"{name}: out_dtype must be q's type or fp32")
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+        out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
     else:
         _need_heads(name, "out", out, out_dtype)
         if out.shape != q.shape:
