@@ -39,7 +39,7 @@
 //   V rows are zeroed in shared memory before the product (0 * NaN would
 //   otherwise reach the result), by the V producer, in the last block of a
 //   sequence only.
-// * Paged: a key block is 128 / page_size copies, one per page (one copy of a
+// * Paged: a key block is 128 (64) / page_size copies, one per page (one copy of a
 //   part of a larger page), issued by as many lanes; page indices are read one
 //   block ahead. An index outside the cache reads zeros and is reported.
 #include "attn_common.cuh"
@@ -851,132 +851,104 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         tc_fence_after();
         // Probabilities are formed against a reference that trails the row's
         // maximum by at most kRescaleThreshold; if a row grows past that, O and l
-        // are brought to a new one. Blocks of 64 (but an item's first) look for
-        // the maximum beside the exponentials, in the exp unit's shadow, and
-        // make a pass that turns out to need a new reference again, from the
-        // scores that still stand in TMEM: one prompt of 16 384 tokens, hd 128,
-        // 1042 -> 980 us. With 128 scores that keeps too much in registers (it
-        // spills, 104 -> 135 us for 8 sequences of 1025 to 2047 tokens).
-        constexpr bool kMaxFirst = C::kBN == 128;
-        uint32_t pk[C::kBN / 2];
-        auto load = [&](float (&s)[C::kBN]) {
-          uint32_t v[C::kBN];
-          if constexpr (C::kBN == 128) {
-            tmem_ld128(tm_s + slot * C::kBN, v);
-          } else {
-            tmem_ld64(tm_s + slot * C::kBN, v);
-          }
+        // are brought to a new one. The maximum is found beside the
+        // exponentials, in the exp unit's shadow, and a pass that turns out to
+        // need a new reference is made again, from the scores that still stand in
+        // TMEM; only an item's first block has its maximum found first. (Always
+        // first: one prompt of 16 384 tokens, hd 128, 1042 us against 960, two
+        // chunks of 2000 tokens over 14 000 keys, hd 64, 304 against 285, two
+        // prompts of 100 tokens 5.7 against 6.2.) 64 scores at a time: all 128 of
+        // an hd 64 block in registers leave no room for the probabilities.
+        const int lim = admit - j * C::kBN;
+        const bool masked = __any_sync(0xffffffffu, lim < C::kBN);
+        auto load = [&](uint32_t (&v)[64], int at) {
+          tmem_ld64(tm_s + slot * C::kBN + at, v);
           tmem_wait_ld();
+          if (masked) {
 #pragma unroll
-          for (int i = 0; i < C::kBN; ++i) s[i] = __uint_as_float(v[i]);
-          const int lim = admit - j * C::kBN;
-          if (__any_sync(0xffffffffu, lim < C::kBN)) {
-#pragma unroll
-            for (int i = 0; i < C::kBN; ++i) s[i] = i < lim ? s[i] : -INFINITY;
+            for (int i = 0; i < 64; ++i) v[i] = at + i < lim ? v[i] : 0xff800000u;  // -inf
           }
         };
-        auto max_of = [&](float (&mx)[8]) {
-          mx[0] = fmax3f(mx[0], mx[1], mx[2]);
-          mx[3] = fmax3f(mx[3], mx[4], mx[5]);
-          return fmax3f(mx[0], mx[3], fmaxf(mx[6], mx[7])) * c;
-        };
-        auto row_max = [&](const float (&s)[C::kBN]) {
-          float mx[8];
+        if (j == 0) {
+          float m = -INFINITY;
+#pragma unroll 1
+          for (int at = 0; at < C::kBN; at += 64) {
+            uint32_t v[64];
+            load(v, at);
+            auto s = [&](int i) { return __uint_as_float(v[i]); };
+            float mx[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) mx[k] = fmax3f(s[k], s[8 + k], s[16 + k]);
+            for (int k = 0; k < 8; ++k) mx[k] = fmaxf(s(k), s(8 + k));
 #pragma unroll
-          for (int b = 24; b < C::kBN - 8; b += 16)
+            for (int b = 16; b < 64; b += 16)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) mx[k] = fmax3f(mx[k], s[b + k], s[b + 8 + k]);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) mx[k] = fmaxf(mx[k], s[C::kBN - 8 + k]);
-          return max_of(mx);
-        };
-        // True if some row has outgrown its reference, after O and l have been
-        // brought to the new one. Rows that are not stored have no vote: results
-        // must not depend on them.
-        auto raise = [&](float m_row) {
-          const bool need = live && m_row > m_ref + kRescaleThreshold;
-          if (!__any_sync(0xffffffffu, need)) return false;
-          const float m_new = fmaxf(m_ref, m_row);
-          const float alpha = m_ref == -INFINITY ? 0.f : ex2_f32(m_ref - m_new);
-          if (!(ok = wait_pv())) return false;
-          tc_fence_after();
-          rescale_o<HD>(tm_o, alpha);
-          l *= alpha;
-          m_ref = m_new;
-          return true;
-        };
-        // Probabilities into pk, and their sum. In chunks of 16 scores: scaling
-        // of the next chunk and sums and packing of the last are issued between
-        // the exponentials, which the exp unit takes one of in 8 cycles. Scaling
-        // and sums two at a time (f32x2). (All of each in turn: 16 ragged prompts
-        // 40.3 us against 39.8, one prompt of 16 384 tokens, hd 128, 1050 against
-        // 1035.)
-        auto probabilities = [&](const float (&s)[C::kBN], float& m_row) {
+              for (int k = 0; k < 8; ++k) mx[k] = fmax3f(mx[k], s(b + k), s(b + 8 + k));
+            mx[0] = fmax3f(mx[0], mx[1], mx[2]);
+            mx[3] = fmax3f(mx[3], mx[4], mx[5]);
+            mx[0] = fmax3f(mx[0], mx[3], fmaxf(mx[6], mx[7]));
+            m = fmaxf(m, mx[0]);
+          }
+          m_ref = m * c;
+        }
+
+        uint32_t pk[C::kBN / 2];
+        while (true) {
+          // Scaling of the next scores, sums and packing of the last are issued
+          // between the exponentials, which the exp unit takes one of in 8
+          // cycles; scaling and sums two at a time (f32x2).
+          constexpr int kAhead = 2;  // pairs; with 4 and 8 the block of 128 spills
           const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-          uint64_t ls[4] = {0ull, 0ull, 0ull, 0ull};
           const uint64_t c2 = pair_of(c, c), m2 = pair_of(-m_use, -m_use);
-          uint64_t x[C::kBN / 2];
-          float mx[8];
+          uint64_t ls[4] = {0ull, 0ull, 0ull, 0ull};
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = fma_f32x2(pair_of(s[2 * i], s[2 * i + 1]), c2, m2);
+          for (int at = 0; at < C::kBN; at += 64) {
+            uint32_t v[64];
+            load(v, at);
+            auto s = [&](int i) { return __uint_as_float(v[i]); };
+            uint64_t x[32];
 #pragma unroll
-          for (int b = 0; b < C::kBN / 2; b += 8) {
+            for (int i = 0; i < kAhead; ++i) x[i] = fma_f32x2(pair_of(s(2 * i), s(2 * i + 1)), c2, m2);
 #pragma unroll
-            for (int i = b; i < b + 8; i += 2) {
+            for (int i = 0; i < 32; i += 2) {
               float e[4];
               split_pair(x[i], e[0], e[1]);
               split_pair(x[i + 1], e[2], e[3]);
 #pragma unroll
               for (int k = 0; k < 4; ++k) e[k] = ex2_f32(e[k]);
-              if (b + 8 < C::kBN / 2) {
-                x[i + 8] = fma_f32x2(pair_of(s[2 * i + 16], s[2 * i + 17]), c2, m2);
-                x[i + 9] = fma_f32x2(pair_of(s[2 * i + 18], s[2 * i + 19]), c2, m2);
+              if (i + kAhead < 32) {
+                const int a = i + kAhead;
+                x[a] = fma_f32x2(pair_of(s(2 * a), s(2 * a + 1)), c2, m2);
+                x[a + 1] = fma_f32x2(pair_of(s(2 * a + 2), s(2 * a + 3)), c2, m2);
               }
-              if constexpr (!kMaxFirst) {
-                const int k = i - b;
-                mx[k] = b == 0 ? fmaxf(s[2 * i], s[2 * i + 1]) : fmax3f(mx[k], s[2 * i], s[2 * i + 1]);
-                mx[k + 1] = b == 0 ? fmaxf(s[2 * i + 2], s[2 * i + 3]) : fmax3f(mx[k + 1], s[2 * i + 2], s[2 * i + 3]);
-              }
-              pk[i] = pack_p<DT>(e[0], e[1]);
-              pk[i + 1] = pack_p<DT>(e[2], e[3]);
+              mx[i & 3] = fmax3f(mx[i & 3], s(2 * i), s(2 * i + 1));
+              mx[(i & 3) + 1] = fmax3f(mx[(i & 3) + 1], s(2 * i + 2), s(2 * i + 3));
+              pk[at / 2 + i] = pack_p<DT>(e[0], e[1]);
+              pk[at / 2 + i + 1] = pack_p<DT>(e[2], e[3]);
               uint64_t& sum = ls[(i >> 1) & 3];
               sum = add_f32x2(sum, add_f32x2(pair_of(e[0], e[2]), pair_of(e[1], e[3])));
             }
           }
-          if constexpr (!kMaxFirst) m_row = max_of(mx);
-          float y[8];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) split_pair(ls[k], y[2 * k], y[2 * k + 1]);
-          return ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
-        };
+          const float m_row = fmaxf(fmax3f(mx[0], mx[1], mx[2]), mx[3]) * c;
 
-        if constexpr (kMaxFirst) {
-          float s[C::kBN];
-          load(s);
-          float m_row = row_max(s);
-          if (j == 0) {
-            m_ref = m_row;
-          } else {
-            raise(m_row);
-            if (!ok) break;
+          // rows that are not stored have no vote: results must not depend on them
+          const bool need = live && m_row > m_ref + kRescaleThreshold;
+          if (!__any_sync(0xffffffffu, need)) {
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) split_pair(ls[k], y[2 * k], y[2 * k + 1]);
+            l += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+            break;
           }
-          l += probabilities(s, m_row);
-        } else {
-          while (true) {
-            float s[C::kBN];
-            load(s);
-            if (j == 0) m_ref = row_max(s);
-            float m_row;
-            const float sum = probabilities(s, m_row);
-            if (!raise(m_row)) {
-              l += sum;
-              break;
-            }  // else once more: no row is past the new references
-          }
-          if (!ok) break;
+          const float m_new = fmaxf(m_ref, m_row);
+          const float alpha = m_ref == -INFINITY ? 0.f : ex2_f32(m_ref - m_new);
+          if (!(ok = wait_pv())) break;
+          tc_fence_after();
+          rescale_o<HD>(tm_o, alpha);
+          l *= alpha;
+          m_ref = m_new;  // no row is past it now: once more, and no further
         }
+        if (!ok) break;
 
         if constexpr (C::kBN == 128) {
           tmem_st64(tm_s + slot * C::kBN, pk);
