@@ -7,7 +7,11 @@
 //
 // The pipeline is that of flash_fwd_tcgen05 (flash_attn.cu): two query tiles
 // per CTA, S = Q K^T into a ring of TMEM slots, softmax with lazy rescaling in
-// registers, P back over its S slot, O += P V from TMEM. What differs:
+// registers, P back over its S slot, O += P V from TMEM. Bound by the exp unit at
+// hd 64 (busy in 72% of the cycles; 8 sequences of 2048, 16 heads: 0.189 ms, 726
+// TFLOP/s) and by the chain of S, softmax and P V at hd 128 (exp unit and tensor
+// pipe both busy in 61%; 4 sequences of 4096, 16 heads over 2, causal: 0.267 ms,
+// 1028 TFLOP/s). What differs:
 //
 // * A tile's 128 rows are (token, query head of the group) pairs, so all query
 //   heads that share a key head read each K and V tile once: a 4-D tensor map
@@ -103,8 +107,8 @@ static_assert(128 * kSeqRegsLow + 256 * kSeqRegsHigh <= kAttnThreads * kRegsLaun
 // a tile's next S waits for its last P V, and the softmax stood for 2050 of 4450
 // cycles a block; with four of 64 the next S is formed meanwhile (one prompt of
 // 16 384 tokens, 16 heads over 2: 1035 us, with two slots 1140).
-// Blocks of 64 for hd 64 too, six slots: 8 sequences of 1025 to 2047 tokens 113
-// us against 104, there is more to do per block and nothing more to hide.
+// Blocks of 64 for hd 64 too, six slots: 8 sequences of 1025 to 2047 tokens 110
+// us against 101, there is more to do per block and nothing more to hide.
 constexpr int seq_block(int hd) { return hd == 64 ? 128 : 64; }
 
 template <int HD>

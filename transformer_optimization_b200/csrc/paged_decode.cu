@@ -12,7 +12,9 @@
 // barrier in the loop, no per-lane addresses), and the products run on
 // mma.sync m16n8k16, whose 16 rows fit the group and whose result layout feeds
 // the probabilities straight back as the next operand (the tcgen05 form needs
-// 128 rows and a TMEM round trip per tile).
+// 128 rows and a TMEM round trip per tile). 32 sequences of 8192 keys, 32 heads
+// over 8, hd 128: 0.179 ms with the join, 5.99 TB/s; 64 of 100 to 8192: 74.5 us;
+// one of 100 000, 16 over 4, hd 64: 24 us; one of 1000: 8 us, all latency.
 //
 // Work is split over keys, not over sequences: all (sequence, key head) items
 // are cut into units of 64 keys, numbered through with kSegment more places
