@@ -12,7 +12,7 @@
 //
 // Bound by HBM: every element is read once and written once, 3 flop each. A
 // block takes a few tokens; its threads first request their rows' vectors
-// (kRows heads per thread, 16 bytes at each end of the pair), then form the
+// (kRotRows heads per thread, 16 bytes at each end of the pair), then form the
 // block's rot/2 angles per token once in shared memory (the fp64 products and
 // sincospif are shared by all heads), then rotate and store. So the angles
 // cost nothing while the loads are in flight: 50 000 tokens, 32 + 2 x 8 heads of
