@@ -344,6 +344,24 @@ def test_packed_bad_offsets_are_reported():
 
 
 @pytest.mark.gpu
+def test_sequences_over_one_another_are_reported():
+    """More tiles than the tokens can hold, with a list, and with tiles cut into key ranges: reported, and in bounds."""
+    k_lens = [9000] + [100] * 79
+    q, k, v, _, cu_k = packed_case([2000], k_lens, 2, 2, 64, F16)
+    cu_q = torch.tensor([0, 2000] * 40 + [0], dtype=torch.int32, device="cuda")
+    for max_k in (1000, 9000):
+        args = (q, k, v, cu_q, cu_k, 2000, 0.125)
+        need = _abi.call_value("tf_flash_packed_workspace", 2000, 80, 2, 2, 64, 2000, max_k)
+        space = torch.full((need + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+        K.flash_attention_packed(*args, max_k=max_k, workspace=space[:need])
+        assert _abi.device_status() == 108
+        assert (space[need:] == 0x5a).all()
+    again = torch.tensor([0, 2000], dtype=torch.int32, device="cuda"), torch.tensor([0, 9000], dtype=torch.int32, device="cuda")
+    out, lse = K.flash_attention_packed(q, k[:9000], v[:9000], *again, 2000, 0.125, want_lse=True, max_k=9000)
+    check_packed(q, k[:9000], v[:9000], *again, 0.125, False, out, lse)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("max_q", [1, 64])
 def test_paged_past_32_bits(max_q):
     """A cache whose pages start past 2^31 elements."""

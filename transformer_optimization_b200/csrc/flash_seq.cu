@@ -244,10 +244,10 @@ __device__ __forceinline__ int block_scan(int x, int* s_warp, int& total) {
 
 // Lists the call's tiles by falling number of key blocks (counting sort over
 // kClasses classes), and sets the item counter to the CTAs' first items. One
-// block. If tiles may be cut and the longest has half as many blocks again as an SM's
-// share of all, tiles longer than half that share become ranges of at most that: at
-// most 2 * total / range = 4 SMs' worth of them, which is what the workspace
-// holds. The order within a class depends on timing, results do not.
+// block. If tiles may be cut and the longest has half as many blocks again as an
+// SM's share of all, tiles longer than half that share become ranges of at most
+// that: fewer than 2 * total / range <= 4 per SM, which is what the workspace
+// holds (a tile of n > range blocks becomes fewer than 2 n / range). The order within a class depends on timing, results do not.
 constexpr int kMinRange = 768;  // keys; a shorter range costs more than it evens out
 constexpr int kCutKeys = 8192;  // keys a sequence may have from which on the call makes room for cuts
 
@@ -365,7 +365,11 @@ __global__ void __launch_bounds__(kPlanThreads) seq_plan_kernel(const __grid_con
         const int slot = atomicAdd(&s_slots, x.ranges);
         const int join = atomicAdd(&s_joins, 1);
         if (slot + x.ranges > p.max_slots || at + x.ranges > p.max_tiles + p.max_slots) {
-          record_error(p.status, kDevBadIndex);  // (cannot be: see above)
+          // more tiles than tokens allow: sequences that lie over one another
+          // (reported above). The list ends here, no entry is left unwritten.
+          x.seq = -1;
+          for (int k = 0; k < x.ranges && at + k < p.max_tiles + p.max_slots; ++k) p.list[at + k] = x;
+          if (join < p.max_slots / 2) p.plan[4 + join] = -1;
           continue;
         }
         p.plan[4 + join] = at;
@@ -1086,7 +1090,9 @@ __global__ void __launch_bounds__(256) seq_combine_kernel(const __grid_constant_
   const int items = (p.plan != nullptr ? p.plan[2] : p.max_tiles) * p.kv_heads * (kRows / 64);
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
     const int head_item = item / (kRows / 64), tile = head_item / p.kv_heads, kvh = head_item - tile * p.kv_heads;
-    const SeqWork w = p.list[p.plan != nullptr ? p.plan[4 + tile] : tile];
+    const int at = p.plan != nullptr ? p.plan[4 + tile] : tile;
+    if (at < 0) continue;
+    const SeqWork w = p.list[at];
     if (w.seq < 0) continue;
     // ranges are kv_heads slots apart; the first is head 0's (list: counted in tiles)
     const long long slot = p.plan != nullptr ? static_cast<long long>(w.slot) * p.kv_heads + kvh : w.slot + kvh;
