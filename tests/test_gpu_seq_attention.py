@@ -386,6 +386,20 @@ def test_paged_past_32_bits(max_q):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_scores_that_grow_from_block_to_block(hd, causal):
+    """Every block outgrows the reference of the one before (for half of the rows; for the others none does)."""
+    q, k, v, cu, _ = packed_case([310], [1000], 4, 2, hd, F16)
+    ramp = torch.arange(1000, device="cuda")[:, None, None] * (0.02 * 64 / hd)
+    k = (0.1 * k.float() + ramp).to(F16)
+    q = (0.1 * q.float() + torch.where(torch.arange(310, device="cuda") % 2 == 0, 1.0, -1.0)[:, None, None]).to(F16)
+    cu_k = torch.tensor([0, 1000], dtype=torch.int32, device="cuda")
+    out, lse = K.flash_attention_packed(q, k, v, cu, cu_k, 310, 0.125, causal=causal, want_lse=True, max_k=1000)
+    check_packed(q, k, v, cu, cu_k, 0.125, causal, out, lse)
+
+
+@pytest.mark.gpu
 def test_large_scores_and_lowest_values():
     """Scores far apart (the running maximum moves by more than 2^8 in later
     blocks), and values at fp16's ends; in bf16 2^20 below them, since the fp32
