@@ -285,6 +285,23 @@ def test_paged(q_lens, kv_lens, h, g, hd, page, causal, dtype):
     check_paged(q, rows, q_lens, hd ** -0.5, causal, out32, None)
 
 
+MANY = [  # more (sequence, key head, row)s than blocks of the join fit on the card
+    ([1] * 120, [1 + 53 * i % 900 for i in range(120)], 16, 4, 128), ([1, 0, 1] * 50, [7 * i % 300 for i in range(150)], 16, 4, 64),
+    ([2, 1] * 150, [11 * i % 257 for i in range(300)], 16, 2, 64), ([3] * 150, [5 + 2 * i for i in range(150)], 20, 4, 128),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_lens,kv_lens,h,g,hd", MANY)
+def test_paged_many_sequences(q_lens, kv_lens, h, g, hd):
+    q, kc, vc, table, cu, lens, rows = paged_case(q_lens, kv_lens, h, g, hd, 16, BF16)
+    args = (q, kc, vc, table, cu, lens, max(q_lens), hd ** -0.5)
+    out, lse = K.flash_attention_paged(*args, want_lse=True, max_kv=max(kv_lens))
+    check_paged(q, rows, q_lens, hd ** -0.5, True, out, lse)
+    again, lse2 = K.flash_attention_paged(*args, want_lse=True, max_kv=max(kv_lens))
+    assert torch.equal(again, out) and torch.equal(lse2, lse)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("max_q", [1, 100])
 def test_paged_rows_outside(max_q):

@@ -13,8 +13,8 @@
 // mma.sync m16n8k16, whose 16 rows fit the group and whose result layout feeds
 // the probabilities straight back as the next operand (the tcgen05 form needs
 // 128 rows and a TMEM round trip per tile). 32 sequences of 8192 keys, 32 heads
-// over 8, hd 128: 0.179 ms with the join, 5.99 TB/s; 64 of 100 to 8192: 74.5 us;
-// one of 100 000, 16 over 4, hd 64: 24 us; one of 1000: 8 us, all latency.
+// over 8, hd 128: 0.178 ms with the join, 6.03 TB/s; 64 of 100 to 8192: 70.3 us;
+// one of 100 000, 16 over 4, hd 64: 23.6 us; one of 1000: 7.5 us, all latency.
 //
 // Work is split over keys, not over sequences: all (sequence, key head) items
 // are cut into units of 64 keys, numbered through with kSegment more places
@@ -52,6 +52,7 @@ struct DecodeK {
   float scale_log2;
   float* o_part;   // [2 * gridDim.x][16][HD]
   float* l_part;   // [2 * gridDim.x][16] log2-sum-exp
+  int2* spans;     // [batch][kv_heads] place of the item's first partial result, blocks that have part in it
   int* status;
 };
 
@@ -316,6 +317,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm)
     const bool whole = c_begin == 0 && c_end == now.nu;
     // the item began before this run: its partial result takes the second place
     const bool earlier = now.left != u_end - u_begin && c_begin == 0;
+    if (c_begin == 0 && threadIdx.x == 0) {
+      const int last = runs.block_of(u_end - now.left + now.nu - 1);
+      p.spans[now.seq * a.kv_heads + kvh] =
+          make_int2(2 * static_cast<int>(blockIdx.x) + (earlier ? 1 : 0), last - static_cast<int>(blockIdx.x) + 1);
+    }
     const int rows = s.q * p.group;
     // keys row r admits: up to its token's own position (causal)
     const int lim0 = a.causal ? s.k - s.q + (lane >> 2) / p.group + 1 : s.k;
@@ -508,67 +514,63 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm)
 
 // Joins the partial results of every item that more than one block worked on,
 // and writes the rows of sequences without keys (out 0, log-sum-exp -inf).
-// One block per (sequence, key head) and row: the weights of all partial
-// results first, then each warp adds up every eighth result, eight of them
-// requested at a time, and the warps' sums are added in warp order. What
-// bounds it is the chain of latencies (lengths, weights, results), so a long
-// join is spread over the warps.
+// One block per (sequence, key head) and ROWS rows, 8 / ROWS warps to each:
+// the maximum first, then each warp adds up its share of the results, eight of
+// them requested at a time, and the warps' sums are added in warp order. What
+// bounds it is the chain of latencies (lengths, maximum, results), so a long
+// join is spread over the warps; a call with more rows than blocks fit on the
+// card takes several to a block. Where an item's partial results are is what
+// the block that began it left in `spans`. (Found from the lengths of all
+// sequences, a row to a block: 200 sequences of 100 keys, 64 heads over 8, hd 64,
+// 83 us against 25, 256 of 600, 32 over 8, hd 128, 150 against 113.)
 constexpr int kJoinWarps = 8;
+constexpr int kJoinCtasPerSm = 8;  // that are resident
 
-template <int HD, int DT>
+template <int HD, int DT, int ROWS>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_combine_kernel(const __grid_constant__ DecodeK p, int blocks) {
   constexpr int E = HD / 32;
-  extern __shared__ float s_w[];  // [blocks] weights
+  extern __shared__ float s_w[];  // [warps][blocks] log-sum-exps of a row's partial results
   __shared__ float s_o[kJoinWarps][HD];
   __shared__ float s_l[kJoinWarps], s_max[kJoinWarps];
   const SeqArgs& a = p.a;
   pdl_wait();
   pdl_trigger();
   const int seq = blockIdx.x / a.kv_heads, kvh = blockIdx.x - seq * a.kv_heads;
-  const int r = blockIdx.y;
   const int lane = lane_id(), warp = warp_id();
+  constexpr int kStep = kJoinWarps / ROWS;  // warps of a row
+  const int r0 = blockIdx.y * ROWS, r = r0 + warp % ROWS;
   const SeqLens s = decode_lens(a, p.group, p.page_shift, seq);
-  if (s.bad && kvh == 0 && r == 0 && threadIdx.x == 0) record_error(p.status, kDevBadIndex);
-  if (r >= s.q * p.group) return;
-  const int nu = units_of(s);
-  int c0 = 0, n = 0;  // the item's blocks
-  bool late = false;
-  if (nu > 0) {
-    int all = 0, mine = 0;  // places of all sequences, and of those before this one
-#pragma unroll 4
-    for (int b = lane; b < a.batch; b += 32) {
-      const int x = places_of(decode_lens(a, p.group, p.page_shift, b));
-      all += x;
-      mine += b < seq ? x : 0;
-    }
-    const Runs runs(__reduce_add_sync(0xffffffffu, all) * a.kv_heads, blocks);
-    const int ua = __reduce_add_sync(0xffffffffu, mine) * a.kv_heads + kvh * (nu + kSegment);
-    c0 = runs.block_of(ua);
-    n = runs.block_of(ua + nu - 1) - c0 + 1;
-    if (n == 1) return;  // one block saw all of it and wrote the result
-    // block c's partial result is in its first place, unless its run began
-    // before the item (only c0's can have)
-    late = runs.start(c0) < ua;
+  if (s.bad && kvh == 0 && r0 == 0 && threadIdx.x == 0) record_error(p.status, kDevBadIndex);
+  const int end = s.q * p.group;
+  if (r0 >= end) return;
+  // An item's first partial result is in the first place of its block, or in
+  // the second if that block's run began before the item; the others are in
+  // the first places of the blocks after it. Items without keys have none.
+  int2 span = make_int2(0, 0);
+  if (units_of(s) > 0) {
+    span = p.spans[blockIdx.x];
+    if (span.y == 1) return;  // one block saw all of it and wrote the result
   }
-  auto part = [&](int i) { return 2ll * (c0 + i) + (late && i == 0 ? 1 : 0); };
+  int n = span.y;
+  auto part = [&](int i) -> long long { return i == 0 ? span.x : (span.x & ~1) + 2 * i; };
+  if (r >= end) n = 0;
   float m = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += kJoinWarps * 32) {
-    s_w[i] = p.l_part[part(i) * kDecRows + r];
-    m = fmaxf(m, s_w[i]);
+  float* lg = s_w + warp * blocks;
+#pragma unroll 4
+  for (int i = lane; i < n; i += 32) {
+    const float x = p.l_part[part(i) * kDecRows + r];
+    lg[i] = x;
+    m = fmaxf(m, x);
   }
+  __syncwarp();
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  if (lane == 0) s_max[warp] = m;
-  __syncthreads();
-  m = s_max[0];
-#pragma unroll
-  for (int w = 1; w < kJoinWarps; ++w) m = fmaxf(m, s_max[w]);
   float l = 0.f, acc[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.f;
 #pragma unroll 8
-  for (int i = warp; i < n; i += kJoinWarps) {
-    const float w = s_w[i] == -INFINITY ? 0.f : ex2_f32(s_w[i] - m);
+  for (int i = warp / ROWS; i < n; i += kStep) {
+    const float w = lg[i] == -INFINITY ? 0.f : ex2_f32(lg[i] - m);
     const float* src = p.o_part + (part(i) * kDecRows + r) * HD + lane * E;
     l += w;
     if constexpr (E == 4) {
@@ -585,27 +587,33 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_combine_kernel(const __
   }
 #pragma unroll
   for (int i = 0; i < E; ++i) s_o[warp][lane * E + i] = acc[i];
-  if (lane == 0) s_l[warp] = l;
+  if (lane == 0) {
+    s_l[warp] = l;
+    s_max[warp] = m;
+  }
   __syncthreads();
-  if (threadIdx.x >= HD) return;
-  float x = 0.f;
-  l = 0.f;
+  for (int i = threadIdx.x; i < ROWS * HD; i += kJoinWarps * 32) {
+    const int row = i / HD, col = i - row * HD;
+    if (r0 + row >= end) return;
+    float x = 0.f;
+    l = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) {
-    l += s_l[w];
-    x += s_o[w][threadIdx.x];
+    for (int w = 0; w < kStep; ++w) {
+      l += s_l[row + w * ROWS];
+      x += s_o[row + w * ROWS][col];
+    }
+    x = l > 0.f ? x / l : 0.f;
+    const int tok = s.q0 + (r0 + row) / p.group, head = kvh * p.group + (r0 + row) % p.group;
+    const long long at = static_cast<long long>(tok) * a.o_ts + static_cast<long long>(head) * a.o_hs + col;
+    if (a.out_f32) {
+      static_cast<float*>(a.out)[at] = x;
+    } else {
+      static_cast<uint16_t*>(a.out)[at] = static_cast<uint16_t>(pack2<DT>(x, 0.f) & 0xffffu);
+    }
+    if (a.lse != nullptr && col == 0)
+      a.lse[static_cast<long long>(head) * a.tokens + tok] =
+          l > 0.f ? (s_max[row] + __log2f(l)) * 0.69314718055994531f : -INFINITY;
   }
-  x = l > 0.f ? x / l : 0.f;
-  const int tok = s.q0 + r / p.group, head = kvh * p.group + r % p.group;
-  const long long at = static_cast<long long>(tok) * a.o_ts + static_cast<long long>(head) * a.o_hs + threadIdx.x;
-  if (a.out_f32) {
-    static_cast<float*>(a.out)[at] = x;
-  } else {
-    static_cast<uint16_t*>(a.out)[at] = static_cast<uint16_t>(pack2<DT>(x, 0.f) & 0xffffu);
-  }
-  if (a.lse != nullptr && threadIdx.x == 0)
-    a.lse[static_cast<long long>(head) * a.tokens + tok] =
-        l > 0.f ? (m + __log2f(l)) * 0.69314718055994531f : -INFINITY;
 }
 
 // Blocks of a call: every SM's share, but no more than there can be units.
@@ -628,10 +636,19 @@ int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeK& k
     attr_done[dev & 63] = true;
   }
   cudaError_t e = launch_k(kern, dim3(blocks), dim3(kDecWarps * 32), C::kBytes, stream, tk, tv, k);
-  if (e == cudaSuccess)
-    e = launch_k(paged_combine_kernel<HD, DT>,
-                 dim3(static_cast<unsigned>(k.a.batch * k.a.kv_heads), static_cast<unsigned>(k.a.max_q * k.group)),
-                 dim3(kJoinWarps * 32), blocks * sizeof(float), stream, k, blocks);
+  if (e == cudaSuccess) {
+    const long long items = k.a.batch * k.a.kv_heads;
+    const int most = static_cast<int>(k.a.max_q * k.group);
+    int rows = 1;  // per join block
+    while (rows < kJoinWarps && rows < most && items * ((most + rows - 1) / rows) > kJoinCtasPerSm * device_sm_count())
+      rows *= 2;
+    auto join = rows == 1   ? paged_combine_kernel<HD, DT, 1>
+                : rows == 2 ? paged_combine_kernel<HD, DT, 2>
+                : rows == 4 ? paged_combine_kernel<HD, DT, 4>
+                            : paged_combine_kernel<HD, DT, 8>;
+    e = launch_k(join, dim3(static_cast<unsigned>(items), (most + rows - 1) / rows), dim3(kJoinWarps * 32),
+                 kJoinWarps * blocks * sizeof(float), stream, k, blocks);
+  }
   if (e != cudaSuccess) return set_error(TF_ERR_LAUNCH, "paged decode launch: %s", cudaGetErrorString(e));
   return TF_OK;
 }
@@ -641,7 +658,7 @@ int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeK& k
 bool paged_is_decode(const SeqArgs& a) { return a.max_q * (a.heads / a.kv_heads) <= kDecRows; }
 
 long long paged_decode_workspace(const SeqArgs& a) {
-  return static_cast<long long>(decode_blocks(a)) * 2 * kDecRows * (a.head_dim + 1) * 4;
+  return static_cast<long long>(decode_blocks(a)) * 2 * kDecRows * (a.head_dim + 1) * 4 + a.batch * a.kv_heads * 8;
 }
 
 int paged_decode(const SeqArgs& a, cudaStream_t stream) {
@@ -655,6 +672,7 @@ int paged_decode(const SeqArgs& a, cudaStream_t stream) {
   const int blocks = decode_blocks(a);
   k.o_part = static_cast<float*>(a.workspace);
   k.l_part = k.o_part + static_cast<long long>(blocks) * 2 * kDecRows * a.head_dim;
+  k.spans = reinterpret_cast<int2*>(k.l_part + static_cast<long long>(blocks) * 2 * kDecRows);
   k.status = device_status_ptr();
   if (k.status == nullptr) return last_error_code();
   CUtensorMap tk, tv;
