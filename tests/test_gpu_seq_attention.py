@@ -403,6 +403,19 @@ def test_paged_past_32_bits(max_q):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("most", [0, 100])
+def test_key_bound_only_sizes_the_split(most):
+    """A bound on the keys that is too small costs time, not results."""
+    q, k, v, cu, cu_k = packed_case([40, 90], [3000, 200], 4, 2, 64, F16)
+    out, lse = K.flash_attention_packed(q, k, v, cu, cu_k, 90, 0.125, causal=True, want_lse=True, max_k=most)
+    check_packed(q, k, v, cu, cu_k, 0.125, True, out, lse)
+    for q_lens in ([1, 1], [40, 9]):
+        q, kc, vc, table, cu, lens, rows = paged_case(q_lens, [3000, 200], 4, 2, 64, 16, F16)
+        out, lse = K.flash_attention_paged(q, kc, vc, table, cu, lens, max(q_lens), 0.125, want_lse=True, max_kv=most)
+        check_paged(q, rows, q_lens, 0.125, True, out, lse)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("causal", [False, True])
 def test_scores_that_grow_from_block_to_block(hd, causal):
