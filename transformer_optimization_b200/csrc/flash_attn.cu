@@ -75,8 +75,8 @@ struct AttnCfg {
   static constexpr int kVOff = kKOff + kKStages * kTileBytes;
   static constexpr int kBarOff = kVOff + kVStages * kTileBytes;
   // q_full, k_full/empty[KS], v_full/empty[VS], s_full[NS],
-  // p_full[2 tiles x 4], turn[2], drain[2], pv_done[NS]
-  static constexpr int kNumBars = 1 + 2 * kKStages + 2 * kVStages + kNS + 8 + 2 + 2 + kNS;
+  // p_full[2 tiles x 4], turn[2], drain[2], pv_done[NS], o_done[2]
+  static constexpr int kNumBars = 1 + 2 * kKStages + 2 * kVStages + kNS + 8 + 2 + 2 + kNS + 2;
   static constexpr int kBytes = kBarOff + kNumBars * 8 + 16;
   static constexpr int kAlloc = kBytes + 1024;
   // TMEM columns: S/P slots at 0, 128, ..; O_t at kNS*128 + t*HD (512 in all)
@@ -155,7 +155,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   uint64_t* turn = p_full + 8;     // exp-phase hand-off between the two softmax warpgroups
   uint64_t* drain = turn + 2;       // [issuer]: end-of-kernel drain of each MMA issuer
   uint64_t* pv_done = drain + 2;    // [slot]: the PV that read this slot's P has completed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + NS);
+  uint64_t* o_done = pv_done + NS;  // [tile]: the tile's last PV has completed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
 
   const int warp = warp_id();
   const int lane = lane_id();
@@ -202,6 +203,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int i = 0; i < 8; ++i) mbar_init(&p_full[i], 128);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&turn[i], 128);
+      mbar_init(&o_done[i], 1);
     }
     mbar_init(&drain[0], 1);
     mbar_init(&drain[1], 1);
@@ -320,6 +322,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             umma_f16_ts(tmem_base + C::kTmO + t * HD, tmem_base + C::kTmS + slot * 128 + k * 8,
                         smem_desc_sw128(va + k * 2048, 16384, 1024), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
           umma_commit(&pv_done[slot]);
+          if (j + 1 == (t == 0 ? nblk[0] : nblk[1])) umma_commit(&o_done[t]);
           if (last_user(t, j)) umma_commit(&v_empty[j % VS]);
         }
       }
@@ -347,10 +350,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
     // issue order of (t, j)
     auto pair_at = [&](int j) { return j < nmin ? 2 * j + t : 2 * nmin + (j - nmin); };
-    // every PV up to the tile's block j has landed in O. The slot's barrier is
-    // exact: S of this thread's newest pair waited for the PV NS pairs back,
-    // so no phase before the awaited one of that slot is open. (One barrier
-    // per tile would not do: with one tile alone its PVs run up to NS behind.)
+    // every PV up to the tile's block j has landed in O, for a thread that has
+    // still to give up P(j + 1). The slot's barrier is exact then: S of this
+    // thread's newest pair waited for the PV NS pairs back, so no phase before
+    // the awaited one of that slot is open, and the slot's next PV follows
+    // PV(j + 1). (One barrier for all of a tile's PVs would not do: with one
+    // tile alone they run up to NS behind.) Behind the last block nothing holds
+    // the other tile's PVs back from coming round to the slot: that wait is on
+    // o_done, which completes once.
     auto wait_pv = [&](int j) {
       const int q = pair_at(j);
       return mbar_wait(&pv_done[q % NS], (q / NS) & 1, p.status, kDevTimeoutSoftmax);
@@ -512,7 +519,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       float inv = 0.f;
       uint32_t ov[HD];
       if (nb > 0) {
-        if (!(ok = wait_pv(nb - 1))) {
+        if (!(ok = mbar_wait(&o_done[t], 0, p.status, kDevTimeoutSoftmax))) {
           // fall through to the barrier; nothing is written
         } else {
           tc_fence_after();
