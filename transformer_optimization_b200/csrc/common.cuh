@@ -46,12 +46,20 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
   return t;
 }
 
+// The first error stays until the host reads it; a bad index, which ends no
+// kernel early, gives way to one that does.
 __device__ __forceinline__ void record_error(int* status, int code) {
-  if (status != nullptr) atomicCAS(status, 0, code);
+  if (status == nullptr) return;
+  if (atomicCAS(status, kDevOk, code) == kDevBadIndex && code != kDevBadIndex) atomicCAS(status, kDevBadIndex, code);
 }
 
+// Whether a wait somewhere ran out, so that others need not. A bad index is
+// no such error: it concerns one call's arguments, and the host may read it
+// many launches later.
 __device__ __forceinline__ bool error_raised(const int* status) {
-  return status != nullptr && *((volatile const int*)status) != 0;
+  if (status == nullptr) return false;
+  const int code = *((volatile const int*)status);
+  return code != kDevOk && code != kDevBadIndex;
 }
 
 // ---------------------------------------------------------------------------
@@ -92,8 +100,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 }
 
 // Wait for the phase with the given parity to complete. Returns false (and
-// records `code`) if it has not completed within kWaitLimitNs, or if another
-// CTA already raised an error. The spin itself only polls the barrier and the
+// records `code`) if it has not completed within kWaitLimitNs, or if a wait
+// of another CTA already ran out. The spin itself only polls the barrier and the
 // SM cycle counter; the device status word (a global-memory read) and the
 // wall clock are looked at every kSlowCheckCycles, so a barrier that
 // completes is seen at once instead of behind a memory round trip.
