@@ -42,7 +42,7 @@ extern "C" {
 #define TF_ERR_UNSUPPORTED 4 /* device is not sm_100 */
 #define TF_ERR_DEVICE 5      /* CUDA runtime error outside a launch */
 #define TF_ERR_DRIVER 6      /* driver entry point (tensor-map encode) */
-#define TF_ERR_TIMEOUT 7     /* a kernel wait ran out (see tf_device_status) */
+#define TF_ERR_TIMEOUT 7     /* a kernel wait ran out, or a bad index was met (see tf_device_status) */
 
 /* tf_ln_residual flags */
 #define TF_LN_MASK_DELTA 1 /* zero invalid rows of delta before the add */
@@ -99,7 +99,10 @@ int tf_abi_version(void);
 const char* tf_last_error(void);
 
 /* Synchronises `stream`, then returns the device status word of the current
- * device in *code (0 = no kernel wait ran out) and clears it.
+ * device in *code and clears it: 0 = nothing to report, 101 .. 107 = a kernel
+ * wait ran out, 108 = a slot, page, length or offset outside its array (read
+ * as the entry point says; later calls are not affected). A wait that runs
+ * out takes the place of a 108 that has not been read.
  * No reference counterpart: the reference's Triton wrappers raise
  * (torch_transformer_benchmark.py:1053-1058) and cannot time out. */
 int tf_device_status(int* code, void* stream);

@@ -73,3 +73,10 @@ def test_index_error_behind_a_wait():
     K.wait_timeout_probe(torch.zeros(4096, dtype=torch.uint8, device="cuda"), 20_000)
     report_bad_slot()
     assert _abi.device_status() == 106
+
+
+def test_status_message_says_what_it_was():
+    report_bad_slot()
+    assert _abi.device_status() == 108
+    message = _abi.load().tf_last_error().decode()
+    assert "index" in message and "108" in message and "wait" not in message

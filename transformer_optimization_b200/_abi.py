@@ -146,7 +146,7 @@ def call_value(fn: str, *args) -> int:
 
 def device_status(stream: int = 0) -> int:
     """Synchronise `stream`, return and clear the device status word
-    (0 = no kernel wait ran out)."""
+    (0 = no kernel wait ran out, and no bad index was met: 108)."""
     code = ctypes.c_int(0)
     rc = load().tf_device_status(ctypes.byref(code), ctypes.c_void_p(stream))
     if rc not in (TF_OK, TF_ERR_TIMEOUT):

@@ -10,6 +10,7 @@
 
 #include <cstdlib>
 
+#include "common.cuh"
 #include "launch.h"
 
 namespace tfb {
@@ -202,6 +203,8 @@ int tf_device_status(int* code, void* stream) {
   e = cudaMemcpyToSymbol(tfb::g_tfb_status, &zero, sizeof(int));
   if (e != cudaSuccess) return set_error(TF_ERR_DEVICE, "clear status: %s", cudaGetErrorString(e));
   *code = host;
+  if (host == tfb::kDevBadIndex)
+    return set_error(TF_ERR_TIMEOUT, "a slot, page, length or offset index outside its array (device code %d)", host);
   return host == 0 ? TF_OK : set_error(TF_ERR_TIMEOUT, "a kernel wait ran out (device code %d)", host);
 }
 
