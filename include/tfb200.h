@@ -333,7 +333,9 @@ int tf_rotary_append(const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int
  * 0 .. i + (keys - queries): its last query stands at its last key. out: q's
  * type (fp32 with TF_ATTN_OUT_F32); lse: fp32 [heads, tokens] natural
  * log-sum-exp or NULL. A query without admissible keys gets out = 0 and
- * lse = -inf; rows of out and lse outside the sequences are left as they were.
+ * lse = -inf (so does one whose every score is -inf); a score of NaN or +inf
+ * makes its row NaN in out and lse, however the keys are split; rows of out and
+ * lse outside the sequences are left as they were.
  * Keys and values of other sequences never reach a result, whatever they hold
  * (a non-finite value of the own sequence reaches the rows of its 128-row tile
  * even where the causal mask hides it). max_q, max_k: host bounds on a

@@ -994,8 +994,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         for (int i = 0; i < HD; ++i) ov[i] = 0u;
       }
       qc += n0 + n1;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      const float lse = l > 0.f ? (m_ref + __log2f(l)) * 0.69314718055994531f : -INFINITY;
+      // a sum of 0 is that of a row without keys (or whose every score is -inf);
+      // one of NaN (a score of NaN or +inf) goes on into the result, the
+      // log-sum-exp and the join
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float lse = l == 0.f ? -INFINITY : (m_ref + __log2f(l)) * 0.69314718055994531f;
       const SeqOut& o = s_out;
       const int slot_out = item->slot;
       if (slot_out >= 0) {
@@ -1128,7 +1131,7 @@ __global__ void __launch_bounds__(256) seq_combine_kernel(const __grid_constant_
         acc[i].w = fmaf(f, y.w, acc[i].w);
       }
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     const long long token = w.q0 + tok;
     const int head = kvh * p.group + (rr - tl * p.group);
     const long long base = token * p.o.o_ts + head * p.o.o_hs + quarter * (HD / 4);
@@ -1145,7 +1148,7 @@ __global__ void __launch_bounds__(256) seq_combine_kernel(const __grid_constant_
                        pack2<DT>(acc[i + 1].x * inv, acc[i + 1].y * inv), pack2<DT>(acc[i + 1].z * inv, acc[i + 1].w * inv));
     }
     if (p.o.lse != nullptr && quarter == 0)
-      p.o.lse[static_cast<long long>(head) * p.o.tokens + token] = l > 0.f ? m + __logf(l) : -INFINITY;
+      p.o.lse[static_cast<long long>(head) * p.o.tokens + token] = l == 0.f ? -INFINITY : m + __logf(l);
   }
 }
 
