@@ -97,7 +97,7 @@ def test_packed_nonfinite(q_lens, k_lens, h, g, at, hd, dtype, causal, kind):
         for i, (a, b) in enumerate(parts):
             if i == at or i % 7 == 0:
                 lost, kept = check(q[a], k[b], v[b], hd ** -0.5, causal, out[a], lse[:, a])
-                assert (lost > 0) == (i == at) and kept > 0
+                assert kept > 0 and (lost > 0) == (i == at) or kind == "inf key" and lost == 0  # (every score -inf)
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -105,6 +105,19 @@ def test_packed_nonfinite(q_lens, k_lens, h, g, at, hd, dtype, causal, kind):
 @pytest.mark.parametrize("q_lens,k_lens,h,g,at", LONG)
 def test_paged_nonfinite(q_lens, k_lens, h, g, at, hd, dtype, kind):
     paged_nonfinite(q_lens, k_lens, h, g, at, hd, dtype, kind, max(max(q_lens), 17))
+
+
+DECODE = [  # at most 16 rows to a key head
+    ([1, 1, 1], [40, 9000, 700], 8, 2, 1), ([1, 1, 1], [40, 9000, 700], 8, 2, 0), ([4, 1, 3], [50, 20, 3000], 8, 2, 2),
+    ([1] * 120, [1 + 53 * i % 900 for i in range(120)], 16, 4, 77), ([2, 1] * 150, [11 * i % 257 + 2 for i in range(300)], 16, 2, 10),
+]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("q_lens,k_lens,h,g,at", DECODE)
+def test_decode_nonfinite(q_lens, k_lens, h, g, at, hd, dtype, kind):
+    paged_nonfinite(q_lens, k_lens, h, g, at, hd, dtype, kind, max(q_lens))
 
 
 def paged_nonfinite(q_lens, k_lens, h, g, at, hd, dtype, kind, max_q):
@@ -120,4 +133,4 @@ def paged_nonfinite(q_lens, k_lens, h, g, at, hd, dtype, kind, max_q):
         for i, (a, (k, v)) in enumerate(zip(parts, rows)):
             if i == at or i % 7 == 0:
                 lost, kept = check(q[a], k, v, hd ** -0.5, True, out[a], lse[:, a])
-                assert (lost > 0) == (i == at) and kept > 0
+                assert kept > 0 and (lost > 0) == (i == at) or kind == "inf key" and lost == 0  # (every score -inf)

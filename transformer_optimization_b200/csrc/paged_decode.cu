@@ -471,8 +471,10 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm)
           f[w] = s_m[w][row] == -INFINITY ? 0.f : ex2_f32(s_m[w][row] - M);
           L += s_l[w][row] * f[w];
         }
-        const float inv = L > 0.f ? 1.f / L : 0.f;
-        const float lg = L > 0.f ? M + __log2f(L) : -INFINITY;
+        // 0: no keys for this row (or every score -inf); NaN goes on into the
+        // result, the log-sum-exp and the join
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float lg = L == 0.f ? -INFINITY : M + __log2f(L);
         const int tok = s.q0 + r / p.group, head = kvh * p.group + r % p.group;
         const int col = threadIdx.x & 15;
         const long long place = 2ll * blockIdx.x + (earlier ? 1 : 0);
@@ -602,7 +604,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_combine_kernel(const __
       l += s_l[row + w * ROWS];
       x += s_o[row + w * ROWS][col];
     }
-    x = l > 0.f ? x / l : 0.f;
+    x = l == 0.f ? 0.f : x / l;
     const int tok = s.q0 + (r0 + row) / p.group, head = kvh * p.group + (r0 + row) % p.group;
     const long long at = static_cast<long long>(tok) * a.o_ts + static_cast<long long>(head) * a.o_hs + col;
     if (a.out_f32) {
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_combine_kernel(const __
     }
     if (a.lse != nullptr && col == 0)
       a.lse[static_cast<long long>(head) * a.tokens + tok] =
-          l > 0.f ? (s_max[row] + __log2f(l)) * 0.69314718055994531f : -INFINITY;
+          l == 0.f ? -INFINITY : (s_max[row] + __log2f(l)) * 0.69314718055994531f;
   }
 }
 
