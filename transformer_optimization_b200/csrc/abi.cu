@@ -619,6 +619,15 @@ int tf_rotary_append(const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int
   return rotary_common("tf_rotary_append", a, heads, kv_heads, head_dim, rot, flags, stream);
 }
 
+// A caller's "no bound" may be any number: bounds past what the arrays can hold
+// (tokens and keys are at most 2^30 and 2^31 - 1, see seq_check) are brought
+// down to that before sizes are computed from them, in the call and in its
+// workspace query alike.
+static void cap_bounds(tfb::SeqArgs& a) {
+  a.max_q = std::min(a.max_q, 1ll << 30);
+  a.max_k = std::min(a.max_k, (1ll << 31) - 1);
+}
+
 static int seq_common(const char* fn, tfb::SeqArgs& a, int64_t heads, int64_t kv_heads, int64_t head_dim, int flags,
                       void* stream) {
   clear_message();
@@ -631,6 +640,7 @@ static int seq_common(const char* fn, tfb::SeqArgs& a, int64_t heads, int64_t kv
   a.causal = (flags & TF_ATTN_CAUSAL) != 0;
   a.out_f32 = (flags & TF_ATTN_OUT_F32) != 0;
   a.bf16 = (flags & TF_ATTN_BF16) != 0;
+  cap_bounds(a);
   rc = tfb::seq_check(a, fn);
   if (rc) return rc;
   rc = begin_call();
@@ -657,6 +667,7 @@ static int64_t seq_workspace_common(const char* fn, int64_t tokens, int64_t batc
   a.o_hs = head_dim;
   a.o_ts = head_dim * heads;
   a.cu_q = a.cu_k = a.kv_lens = reinterpret_cast<const int*>(&a);
+  cap_bounds(a);
   if (tfb::seq_check(a, fn)) return -1;
   if (begin_call()) return -1;
   return tfb::seq_workspace(a);
