@@ -280,7 +280,7 @@ int rotary_check(const RotaryArgs& a, const char* fn) {
                           static_cast<const void*>(a.slots)})
     if (reinterpret_cast<uintptr_t>(ptr) % 8)
       return set_error(TF_ERR_ALIGN, "%s: positions, freqs and slots must be 8-byte aligned", fn);
-  if (!rows_apart(a.head_dim, {{a.qo_ts, a.tokens}, {a.qo_hs, a.heads}}) ||
+  if ((a.heads && !rows_apart(a.head_dim, {{a.qo_ts, a.tokens}, {a.qo_hs, a.heads}})) ||
       (a.kv_heads && !cache && !rows_apart(a.head_dim, {{a.ko_ts, a.tokens}, {a.ko_hs, a.kv_heads}})) ||
       (cache && !rows_apart(a.head_dim, {{a.c_ps, a.num_pages}, {a.c_ts, a.page_size}, {a.c_hs, a.kv_heads}})))
     return set_error(TF_ERR_SHAPE, "%s: rows of an output overlap", fn);
