@@ -263,13 +263,16 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm)
     return x.left > 0 && key0 < x.s.k ? a.page_table[x.seq * a.table_ld + (key0 >> p.page_shift)] : 0;
   };
   int page = page_of(ahead);
+  bool ok = true;       // false: a wait of this warp ran out; it loads and takes no more tiles, its results are NaN
+  uint32_t loaded = 0;  // bit i: stage i has a tile on its way or not yet taken
   auto load_next = [&](int stage) {
-    if (ahead.left <= 0) return;
+    if (ahead.left <= 0 || !ok) return;
     const int key0 = ahead.c * kDecUnit + warp * kDecTile;
+    if (key0 < ahead.s.k) loaded |= 1u << stage;
     if (key0 < ahead.s.k && lane == 0) {
-      const bool ok = page >= 0 && page < a.num_pages;
-      if (!ok) record_error(p.status, kDevBadIndex);
-      const int z = ok ? page : (1 << 30);  // past every cache: zeros
+      const bool held = page >= 0 && page < a.num_pages;
+      if (!held) record_error(p.status, kDevBadIndex);
+      const int z = held ? page : (1 << 30);  // past every cache: zeros
       const int row = key0 & ((1 << p.page_shift) - 1);
       uint8_t* dst = ring + stage * kStageBytes;
       mbar_arrive_expect_tx(&full[stage], kStageBytes);
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm)
     const int lim1 = a.causal ? s.k - s.q + ((lane >> 2) + 8) / p.group + 1 : s.k;
     const int lim_min = a.causal ? s.k - s.q + 1 : s.k;
 
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = ok ? 0.f : NAN, l1 = l0;
     float o[HD / 8][4];
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i)
@@ -339,9 +342,14 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm)
       __syncwarp();           // every lane is done with the tile before this one:
       load_next(free_stage);  // its stage is refilled
       const int key0 = c * kDecUnit + warp * kDecTile;
-      if (key0 < s.k) {
-        mbar_wait(&full[stage], (parity >> stage) & 1, p.status, kDevTimeoutProducer);
+      if (key0 < s.k && ok &&
+          !__all_sync(0xffffffffu, mbar_wait(&full[stage], (parity >> stage) & 1, p.status, kDevTimeoutProducer))) {
+        ok = false;
+        l0 = l1 = NAN;
+      }
+      if (key0 < s.k && ok) {
         parity ^= 1u << stage;
+        loaded &= ~(1u << stage);
         uint8_t* tile = ring + stage * kStageBytes;
         const uint32_t kt = smem_u32(tile);
         const uint32_t vt = kt + C::kTileBytes;
@@ -512,6 +520,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm)
       }
     }
   }
+  // after a wait that ran out: the copies still on their way land before the
+  // block's memory is given up (bounded, whatever the status says)
+  if (!ok)
+    for (int i = 0; i < C::kStages; ++i)
+      if (loaded >> i & 1) mbar_wait(&full[i], (parity >> i) & 1, nullptr, kDevTimeoutDrain);
 }
 
 // Joins the partial results of every item that more than one block worked on,
