@@ -339,16 +339,21 @@ int tf_rotary_append(const void* q, int64_t q_ts, int64_t q_hs, void* q_out, int
  * Keys and values of other sequences never reach a result, whatever they hold
  * (a non-finite value of the own sequence reaches the rows of its 128-row tile
  * even where the causal mask hides it). max_q, max_k: host bounds on a
- * sequence's queries and keys (max_k only sizes the key split). Lengths or
+ * sequence's queries and keys (max_k only sizes the key split and its
+ * workspace; any larger number is the same as none). Lengths or
  * offsets outside the arrays, or queries past max_q, are cut to the bound and
- * set device code 108. head_dim 64 or 128; heads a multiple of kv_heads, at
+ * set device code 108. Scores, sums and partial results are fp32; the
+ * probabilities are rounded to q's type for the second product, with
+ * TF_ATTN_OUT_F32 too, as in tf_flash_fwd. They are formed against a reference
+ * up to 2^8 below the maximum, so values within a factor of 2^8 * keys of
+ * fp32's largest (bf16 only) may overflow. head_dim 64 or 128; heads a multiple of kv_heads, at
  * most 128 times; scale > 0; bases 16-byte aligned, strides multiples of 8; no
  * two rows of out may overlap, nor out and an operand.
  * workspace: tf_flash_packed_workspace bytes (the same sizes, tokens = q's
  * rows), 16-byte aligned; calls that overlap in time need their own.
- * Replaces the attention of the reference's fp16 path for ragged batches,
- * which it runs padded under a key mask (torch_transformer_benchmark.py:
- * 4146-4161). */
+ * The attention of the reference's fp16 path (torch_transformer_benchmark.py:
+ * 4146-4161) for ragged batches without their padding; the reference, and this
+ * package's models, run those padded under a key mask. */
 int64_t tf_flash_packed_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                   int64_t max_q, int64_t max_k);
 int tf_flash_packed(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,

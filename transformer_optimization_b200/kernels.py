@@ -409,7 +409,10 @@ def attn_merge(o_acc: torch.Tensor, lse_acc: torch.Tensor, o_part: torch.Tensor,
 # ------------------------------------------------- serving: positions and cache
 # The wrappers below check shapes, types and strides before they look for a
 # device, so a malformed call is refused the same way on any host; they run on
-# the tensors' own device and that device's current stream.
+# the tensors' own device and that device's current stream. Like every wrapper
+# here they are forward only: results carry no gradient, whatever the inputs
+# require. An index on the device that points outside its array touches nothing
+# and sets the device status (108, _abi.device_status); later calls run as ever.
 
 
 def _device_of(name: str, first: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
@@ -465,7 +468,10 @@ def rotary_freqs(rot: int, base: float = 10000.0, *, scaling: str = "none", fact
     length): "linear" f_i / factor; "ntk" base * factor^(rot / (rot - 2)), which
     keeps f_0 and divides the last f by factor; "parts" keeps the f_i that turn 32 times or more
     within trained_len, divides those that turn once or less by factor, and
-    blends in between, with mscale = 0.1 ln(factor) + 1."""
+    blends in between linearly in the number of turns, with mscale =
+    0.1 ln(factor) + 1. A checkpoint trained with another table (other cut-offs,
+    or a blend linear in i) needs that table: `rotary` takes any freqs and
+    mscale."""
     if rot < 2 or rot % 2:
         raise ValueError(f"rotary_freqs: rot={rot} must be even and positive")
     if scaling not in ("none", "linear", "ntk", "parts"):
@@ -634,13 +640,17 @@ def flash_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu
     q [T, H, hd], k and v [Tk, KVH, hd]: fp16 or bf16 views with unit inner
     stride (head slices of a packed QKV buffer); query head h reads key head
     h // (H // KVH). Sequence b has queries cu_q[b]:cu_q[b + 1] and keys
-    cu_k[b]:cu_k[b + 1] (int32 [B + 1]); max_q and max_k bound their lengths
-    (max_k, Tk if None, only decides how far the keys are split). causal:
-    query i sees keys up to i + (keys - queries). Returns (out [T, H, hd], lse
-    fp32 [H, T] or None); rows outside the sequences are left as they were, a
-    query without keys gets 0 and -inf. With out_dtype fp32 the results of
-    key ranges merge by attn_merge (a batch of one). workspace (allocated if
-    None) must not serve two calls at a time."""
+    cu_k[b]:cu_k[b + 1] (int32 [B + 1]); max_q and max_k bound their lengths.
+    max_k (Tk if None) only decides how far the keys are split; from 8192 on
+    the call makes room for that (39 MB at hd 64, 78 MB at hd 128) and launches
+    the join, so give the real bound. causal: query i sees keys up to
+    i + (keys - queries). Returns (out [T, H, hd], lse fp32 [H, T] or None);
+    rows outside the sequences are left as they were, a query without keys
+    gets 0 and -inf, one with a score of NaN or +inf gets NaN in both. The
+    probabilities are rounded to q's type for the second product whatever
+    out_dtype is; with fp32 the results of key ranges merge by attn_merge (a
+    batch of one). workspace (allocated if None) must not serve two calls at a
+    time."""
     name = "flash_attention_packed"
     _need_heads(name, "q", q, q.dtype)
     _need_heads(name, "k", k, q.dtype)
@@ -677,8 +687,8 @@ def flash_attention_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     keys of sequence b, its new tokens' (rotary_append) among them, are the
     first kv_lens[b] rows of its pages. Table entries past the last page are
     not read. max_kv bounds kv_lens (the table's capacity if None; it only
-    decides how far the keys are split). Returns (out, lse) as
-    flash_attention_packed."""
+    decides how far the keys are split, as max_k of flash_attention_packed).
+    Returns (out, lse) as flash_attention_packed."""
     name = "flash_attention_paged"
     _need_heads(name, "q", q, q.dtype)
     _need_cache(name, k_cache, v_cache, q, q.shape[2])
