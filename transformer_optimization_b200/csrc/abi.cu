@@ -15,9 +15,10 @@
 
 namespace tfb {
 
-// Status word written by kernels whose bounded waits ran out. One per device
-// (every device that loads this library holds its own copy).
-__device__ int g_tfb_status = 0;
+// Status words written by kernels whose bounded waits ran out, or that met a
+// bad index (common.cuh). One set per device (every device that loads this
+// library holds its own copy).
+__device__ int g_tfb_status[kStatusWords] = {};
 
 namespace {
 thread_local char g_msg[512] = "";
@@ -196,12 +197,13 @@ int tf_device_status(int* code, void* stream) {
   if (code == nullptr) return set_error(TF_ERR_SHAPE, "tf_device_status: code is NULL");
   cudaError_t e = cudaStreamSynchronize(as_stream(stream));
   if (e != cudaSuccess) return set_error(TF_ERR_DEVICE, "stream synchronize: %s", cudaGetErrorString(e));
-  int host = 0;
-  e = cudaMemcpyFromSymbol(&host, tfb::g_tfb_status, sizeof(int));
+  int words[tfb::kStatusWords] = {};
+  e = cudaMemcpyFromSymbol(words, tfb::g_tfb_status, sizeof(words));
   if (e != cudaSuccess) return set_error(TF_ERR_DEVICE, "read status: %s", cudaGetErrorString(e));
-  const int zero = 0;
-  e = cudaMemcpyToSymbol(tfb::g_tfb_status, &zero, sizeof(int));
+  const int zero[tfb::kStatusWords] = {};
+  e = cudaMemcpyToSymbol(tfb::g_tfb_status, zero, sizeof(zero));
   if (e != cudaSuccess) return set_error(TF_ERR_DEVICE, "clear status: %s", cudaGetErrorString(e));
+  const int host = words[0] != 0 ? words[0] : words[1];
   *code = host;
   if (host == tfb::kDevBadIndex)
     return set_error(TF_ERR_TIMEOUT, "a slot, page, length or offset index outside its array (device code %d)", host);

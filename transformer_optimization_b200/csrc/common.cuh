@@ -46,20 +46,22 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
   return t;
 }
 
-// The first error stays until the host reads it; a bad index, which ends no
-// kernel early, gives way to one that does.
+// status[0]: the code of the first wait that ran out, until the host reads it.
+// status[1]: kDevBadIndex if one was met. Apart, since a bad index concerns one
+// call's arguments and must not end the waits of others (error_raised), and
+// since the host may read it many launches later, behind an error of a wait.
+constexpr int kStatusWords = 2;
+
 __device__ __forceinline__ void record_error(int* status, int code) {
-  if (status == nullptr) return;
-  if (atomicCAS(status, kDevOk, code) == kDevBadIndex && code != kDevBadIndex) atomicCAS(status, kDevBadIndex, code);
+  if (status != nullptr) atomicCAS(status, 0, code);
 }
 
-// Whether a wait somewhere ran out, so that others need not. A bad index is
-// no such error: it concerns one call's arguments, and the host may read it
-// many launches later.
+__device__ __forceinline__ void record_bad_index(int* status) {
+  if (status != nullptr) *(static_cast<volatile int*>(status) + 1) = kDevBadIndex;
+}
+
 __device__ __forceinline__ bool error_raised(const int* status) {
-  if (status == nullptr) return false;
-  const int code = *((volatile const int*)status);
-  return code != kDevOk && code != kDevBadIndex;
+  return status != nullptr && *((volatile const int*)status) != 0;
 }
 
 // ---------------------------------------------------------------------------

@@ -179,7 +179,7 @@ __device__ __forceinline__ SeqWork find_tile(const SeqK& p, int at) {
     if (b < p.batch) {
       w = seq_lens<PAGED>(p, b, bad);
       n = (w.q_len + span - 1) / span;
-      if (bad) record_error(p.status, kDevBadIndex);
+      if (bad) record_bad_index(p.status);
     }
     int inc = n;
 #pragma unroll
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kPlanThreads) seq_plan_kernel(const __grid_con
   for (int b = tid; b < p.batch; b += kPlanThreads) {
     bool bad;
     const SeqWork w = seq_lens<PAGED>(p, b, bad);
-    if (bad) record_error(p.status, kDevBadIndex);
+    if (bad) record_bad_index(p.status);
     if (w.q_len > 0) {
       const int last = tile_blocks(p, w, (w.q_len - 1) / p.tok_tile * p.tok_tile);
       most = max(most, last);
@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       int y, z;
       if constexpr (PAGED) {
         const bool ok = page >= 0 && page < p.num_pages;
-        if (!ok) record_error(p.status, kDevBadIndex);
+        if (!ok) record_bad_index(p.status);
         y = (key + lane * rows) & ((1 << p.page_shift) - 1);
         z = ok ? page : (1 << 30);  // past every cache: zeros
       } else {

@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, kDecCtasPerSm)
     if (key0 < ahead.s.k) loaded |= 1u << stage;
     if (key0 < ahead.s.k && lane == 0) {
       const bool held = page >= 0 && page < a.num_pages;
-      if (!held) record_error(p.status, kDevBadIndex);
+      if (!held) record_bad_index(p.status);
       const int z = held ? page : (1 << 30);  // past every cache: zeros
       const int row = key0 & ((1 << p.page_shift) - 1);
       uint8_t* dst = ring + stage * kStageBytes;
@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_combine_kernel(const __
   constexpr int kStep = kJoinWarps / ROWS;  // warps of a row
   const int r0 = blockIdx.y * ROWS, r = r0 + warp % ROWS;
   const SeqLens s = decode_lens(a, p.group, p.page_shift, seq);
-  if (s.bad && kvh == 0 && r0 == 0 && threadIdx.x == 0) record_error(p.status, kDevBadIndex);
+  if (s.bad && kvh == 0 && r0 == 0 && threadIdx.x == 0) record_bad_index(p.status);
   const int end = s.q * p.group;
   if (r0 >= end) return;
   // An item's first partial result is in the first place of its block, or in

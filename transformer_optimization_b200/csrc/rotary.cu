@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryK p) {
           if (page < a.num_pages) {
             off = page * a.c_ps + (slot - page * a.page_size) * a.c_ts;
           } else if (blockIdx.y == 0) {
-            record_error(p.status, kDevBadIndex);
+            record_bad_index(p.status);
           }
         }
       }
